@@ -17,7 +17,8 @@ FORWARD, INVERSE = 0, 1
 MEM_HOST, MEM_DEVICE = 0, 1
 CONV_AUTO, CONV_DIRECT, CONV_OVERLAP_SAVE, CONV_DIRECT_VALU = 0, 1, 2, 3
 IIR_AUTO, IIR_BATCH, IIR_SCAN, IIR_BATCH_REF = 0, 1, 2, 3
-F32, F64 = 0, 1
+F32, F64, F16, BF16 = 0, 1, 2, 3
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 DIST_TRANSPOSED_OUT = 1
 DIST_SERIAL = 2
 
@@ -38,6 +39,11 @@ EXPORTS = (
     "dsp_gpu_iir_multi_ex",
     "dsp_gpu_iir_settle",
     "dsp_gpu_biquad_swept",
+    "dsp_gpu_rotary",
+    "dsp_gpu_linear_attention_workspace",
+    "dsp_gpu_linear_attention",
+    "dsp_gpu_linear_attention_backward",
+    "dsp_gpu_linear_attention_step",
     "dsp_gpu_device_count",
     "dsp_gpu_last_error_string",
     "dsp_gpu_shutdown",
@@ -59,6 +65,15 @@ EXPORTS = (
 
 # dsp_gpu_exchange_fn: (user, send, recv, block_bytes, world, stream) -> status
 EXCHANGE_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p)
+
+
+class LinearAttentionShape(C.Structure):
+    """dsp_gpu_linear_attention_shape"""
+    _fields_ = [("batch", C.c_size_t), ("n", C.c_size_t), ("rows", C.c_size_t),
+                ("heads", C.c_int), ("heads_q", C.c_int), ("heads_k", C.c_int), ("heads_v", C.c_int),
+                ("dim_k", C.c_int), ("dim_v", C.c_int), ("sample_type", C.c_int),
+                ("q_stride", C.c_longlong * 3), ("k_stride", C.c_longlong * 3), ("v_stride", C.c_longlong * 3),
+                ("o_stride", C.c_longlong * 3), ("offsets", C.c_void_p), ("lengths", C.c_void_p), ("zero_rest", C.c_int)]
 
 
 class DspGpuError(RuntimeError):
@@ -104,6 +119,15 @@ def lib() -> C.CDLL:
         L.dsp_gpu_iir_multi_ex.restype = i
         L.dsp_gpu_biquad_swept.argtypes = [vp, vp, vp, sz, sz, sz, i, C.c_double, vp, i, vp]
         L.dsp_gpu_biquad_swept.restype = i
+        ll, d, shape = C.c_longlong, C.c_double, C.POINTER(LinearAttentionShape)
+        L.dsp_gpu_rotary.argtypes = [vp, vp, i, sz, sz, i, i, vp, vp, vp, i, i, vp, vp, ll, d, i, vp]
+        L.dsp_gpu_linear_attention_workspace.argtypes = [shape, i, C.POINTER(sz)]
+        L.dsp_gpu_linear_attention.argtypes = [vp, vp, vp, vp, shape, vp, d, vp, vp, vp, sz, vp]
+        L.dsp_gpu_linear_attention_backward.argtypes = [vp] * 7 + [shape, vp, d, vp, vp, vp, vp, sz, vp]
+        L.dsp_gpu_linear_attention_step.argtypes = [vp, vp, vp, vp, shape, vp, d, vp, vp, sz, vp]
+        for name in ("dsp_gpu_rotary", "dsp_gpu_linear_attention_workspace", "dsp_gpu_linear_attention",
+                     "dsp_gpu_linear_attention_backward", "dsp_gpu_linear_attention_step"):
+            getattr(L, name).restype = i
         L.dsp_gpu_fft_columns.argtypes = [vp, vp, i, sz, i, vp]
         L.dsp_gpu_swap_axes.argtypes = [vp, vp, sz, sz, sz, i, sz, i, vp]
         L.dsp_gpu_transpose_blocks.argtypes = [vp, vp, sz, sz, sz, vp]

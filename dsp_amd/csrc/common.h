@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <functional>
@@ -35,6 +36,22 @@ inline int check_launch(const char *what) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(DSP_GPU_EHIP, "launch of %s failed: %s", what, hipGetErrorString(e));
     return DSP_GPU_OK;
+}
+
+// Whether no two elements of a strided [batch][n][heads][dim] array share an address: taken by stride, each axis steps over
+// the ones inside it.
+inline bool rows_distinct(const long long *stride, size_t batch, size_t n, size_t heads, size_t dim) {
+    struct Axis {
+        size_t stride, count;
+    } ax[3] = {{static_cast<size_t>(stride[0]), batch}, {static_cast<size_t>(stride[1]), n}, {static_cast<size_t>(stride[2]), heads}};
+    std::sort(ax, ax + 3, [](const Axis &x, const Axis &y) { return x.stride < y.stride; });
+    size_t inner = dim;
+    for (const Axis &x : ax) {
+        if (x.count <= 1) continue;
+        if (x.stride < inner) return false;
+        inner = x.stride * (x.count - 1) + inner;
+    }
+    return true;
 }
 
 // ---- streaming helpers shared by the kernels (device side) ------------------------------------
@@ -80,7 +97,7 @@ __device__ __forceinline__ size_t xcd_tile_of(unsigned block, size_t chunk) {
 // never share scratch memory (capi.hip).  Slots keep independent users (host staging in/out, FFT scratch, ...) of one
 // call from aliasing.  `s` is the stream the caller launches on.
 enum WorkspaceSlot {
-    WS_STAGE_IN = 0, WS_STAGE_OUT, WS_SCRATCH_A, WS_SCRATCH_B, WS_STATE, WS_STATE_SNAP, WS_IIR_TABLE, WS_FIR_HIST, WS_COUNTERS, WS_SLOTS
+    WS_STAGE_IN = 0, WS_STAGE_OUT, WS_SCRATCH_A, WS_SCRATCH_B, WS_STATE, WS_STATE_SNAP, WS_IIR_TABLE, WS_FIR_HIST, WS_COUNTERS, WS_ATTENTION, WS_SLOTS
 };
 int workspace(WorkspaceSlot slot, size_t bytes, void **ptr, hipStream_t s);
 // Lets kernel `fn` use up to the CU's whole 160 KiB of dynamic LDS; issued once per kernel and device, not per launch.

@@ -1,0 +1,668 @@
+// linear_attention.hip -- linear attention with a decay for each head: entry points, the plan of a call, and the small
+// kernels around linear_attention_core.h (joining segments, adding up shared heads' gradients, the single-token step).
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <initializer_list>
+
+#include "linear_attention_core.h"
+
+namespace dspgpu {
+namespace la {
+namespace {
+
+// ---- segments -> states ------------------------------------------------------------------------------------------------
+
+// seg[s] holds what segment s leaves behind from a zero state; afterwards it holds the state segment s starts from, and
+// s_out the state after the last one.  One thread an element of the state; the loads do not depend on the recurrence.
+__global__ void __launch_bounds__(256) join_segments_kernel(const Args a) {
+    const Role &role = a.role[blockIdx.y];
+    const int count = role.d1 * role.d2, blocks = (count + 255) / 256;
+    const int bh = blockIdx.x / blocks, e = (blockIdx.x % blocks) * 256 + threadIdx.x;
+    if (bh >= a.batch * a.heads || e >= count) return;
+    long long start, len;
+    sequence_rows(a, bh / a.heads, start, len);
+    const float log2w = a.log2_decay[bh % a.heads];
+    float run = 0.0f;
+    if (role.s_in) run = role.s_in[static_cast<size_t>(bh) * count + (e / role.d2) * role.s_in_d + (e % role.d2) * role.s_in_n];
+    float *seg = role.seg + static_cast<size_t>(bh) * a.segments * count + e;
+    const Decay whole = decay_over(log2w, a.seg_len);
+    for (int s0 = 0; s0 < a.segments; s0 += 8) {
+        float local[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)  // the last segment's own state is computed only where someone asks for it
+            local[i] = s0 + i < a.segments - (role.s_out ? 0 : 1) && (s0 + i) * a.seg_len < len ? seg[static_cast<size_t>(s0 + i) * count] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const long long left = len - (s0 + i) * a.seg_len;
+            if (s0 + i >= a.segments || left <= 0) break;
+            seg[static_cast<size_t>(s0 + i) * count] = run;
+            const Decay w = left >= a.seg_len ? whole : decay_over(log2w, left);
+            run = fmaf(run, w.hi, fmaf(run, w.lo, local[i]));
+        }
+    }
+    if (role.s_out) role.s_out[static_cast<size_t>(bh) * count + e] = run;
+}
+
+// ---- gradients of shared heads -----------------------------------------------------------------------------------------
+
+// Whether a sequence holds `row` (of [batch][n], or of the packed batch) -- what the kernel above wrote.
+__device__ __forceinline__ bool row_taken(const Args &a, long long row) {
+    long long start, len;
+    if (a.offsets) {  // the last sequence that starts at or before it
+        int lo = 0, hi = a.batch - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (a.offsets[mid] <= row) lo = mid;
+            else hi = mid - 1;
+        }
+        sequence_rows(a, lo, start, len);
+        return row >= start && row < start + len;
+    }
+    sequence_rows(a, static_cast<int>(row / a.n), start, len);
+    return row % a.n < len;
+}
+
+// part [row][heads][dim] fp32 -> out [row][heads / group][dim], heads of a group added in their order
+template <typename T>
+__global__ void __launch_bounds__(256) add_heads_kernel(const Args a, const float *part, T *out, int group, int dim) {
+    const long long row = blockIdx.x;
+    if (!row_taken(a, row)) return;
+    const int heads = a.heads / group;
+    for (int e = threadIdx.x; e < heads * dim; e += 256) {
+        const float *p = part + (row * a.heads + (e / dim) * group) * dim + e % dim;
+        float sum = 0.0f;
+        for (int h = 0; h < group; ++h) sum += p[static_cast<size_t>(h) * dim];
+        out[row * heads * dim + e] = static_cast<T>(sum);
+    }
+}
+
+// ---- rows of no sequence -----------------------------------------------------------------------------------------------
+
+struct Rest {
+    void *p[3];
+    long long stride[3][3];
+    int heads[3], dim[3];
+    int wide;  // 4-byte samples
+    long long rows;
+};
+
+// zeros into the rows that no sequence holds (all samples are zero where their bits are)
+__global__ void __launch_bounds__(256) zero_rest_kernel(const Args a, const Rest z) {
+    const int i = blockIdx.y;
+    for (long long row = blockIdx.x; row < z.rows; row += gridDim.x) {
+        if (row_taken(a, row)) continue;
+        const long long at = a.offsets ? row * z.stride[i][1] : row / a.n * z.stride[i][0] + row % a.n * z.stride[i][1];
+        for (int e = threadIdx.x; e < z.heads[i] * z.dim[i]; e += 256) {
+            const long long to = at + e / z.dim[i] * z.stride[i][2] + e % z.dim[i];
+            if (z.wide) static_cast<unsigned *>(z.p[i])[to] = 0;
+            else static_cast<unsigned short *>(z.p[i])[to] = 0;
+        }
+    }
+}
+
+int zero_rest(const Args &a, Rest &z, int count, hipStream_t s) {
+    zero_rest_kernel<<<dim3(static_cast<unsigned>(std::min<long long>(z.rows, 2048)), count), 256, 0, s>>>(a, z);
+    return check_launch("zero_rest_kernel");
+}
+
+// ---- one token ---------------------------------------------------------------------------------------------------------
+
+struct StepArgs {
+    const void *q, *k, *v;
+    void *o;
+    long long qs[2], ks[2], vs[2], os[2];  // strides: row, head
+    int q_group, k_group, v_group;
+    int heads, d1, d2, batch;
+    float scale;
+    int vec;                               // states in 16-byte accesses
+    float *state;                          // [slots][heads][d1][d2]
+    const long long *slots;                // or null: row b has state b
+    long long n_slots;
+    float decay_hi[kMaxHeads], decay_lo[kMaxHeads];  // the decay to 48 bits: rounded to 24 it would drift over long answers
+};
+
+constexpr int kStepCols = 64;
+
+// S <- w S + k v^T, o = scale q S.  Bound by the state's traffic (8 d1 d2 bytes a head): a workgroup takes 64 columns of one
+// head, each thread four columns of every 16th row, all its rows in flight at once.
+// A slot that several rows name is taken by the workgroup of the first of them, for all of them in their order.
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
+    __shared__ float part[4][kStepCols];
+    __shared__ int first, more;
+    const int tiles = (a.d2 + kStepCols - 1) / kStepCols;
+    const int tile = blockIdx.x % tiles, head = blockIdx.x / tiles % a.heads;
+    int b = blockIdx.x / tiles / a.heads;
+    const int tid = threadIdx.x, cx = tid & 15, ry = tid >> 4, lane = tid & 63, wave = tid >> 6;
+    const int n0 = tile * kStepCols + 4 * cx;
+
+    long long slot = b;
+    if (a.slots) {
+        slot = a.slots[b];
+        if (slot < 0 || slot >= a.n_slots) {  // an empty row
+            if (tid < kStepCols && tile * kStepCols + tid < a.d2)
+                static_cast<T *>(a.o)[b * a.os[0] + head * a.os[1] + tile * kStepCols + tid] = static_cast<T>(0.0f);
+            return;
+        }
+    }
+    const float w = a.decay_hi[head], w_lo = a.decay_lo[head];
+    float *state = a.state + ((slot * a.heads + head) * a.d1) * a.d2 + n0;
+    f32x4 s[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int d = ry + 16 * i;
+        s[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (d < a.d1) {
+            if (a.vec) {
+                if (n0 < a.d2) s[i] = *reinterpret_cast<const f32x4 *>(state + static_cast<size_t>(d) * a.d2);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (n0 + c < a.d2) s[i][c] = state[static_cast<size_t>(d) * a.d2 + c];
+            }
+        }
+    }
+    bool again = false;
+    if (a.slots) {
+        if (tid == 0) {
+            first = b;
+            more = 0;
+        }
+        __syncthreads();
+        for (int r = tid; r < a.batch; r += 256)
+            if (r != b && a.slots[r] == slot) {
+                if (r < b) first = r;  // any earlier row: this workgroup is not the slot's
+                else more = 1;
+            }
+        __syncthreads();
+        if (first != b) return;
+        again = more != 0;
+    }
+    for (;;) {
+        const T *q = static_cast<const T *>(a.q) + b * a.qs[0] + (head / a.q_group) * a.qs[1];
+        const T *k = static_cast<const T *>(a.k) + b * a.ks[0] + (head / a.k_group) * a.ks[1];
+        const T *v = static_cast<const T *>(a.v) + b * a.vs[0] + (head / a.v_group) * a.vs[1] + n0;
+        f32x4 vv, acc = {};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) vv[c] = n0 + c < a.d2 ? static_cast<float>(v[c]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int d = ry + 16 * i;
+            if (d < a.d1) {
+                s[i] = s[i] * w + (s[i] * w_lo + static_cast<float>(k[d]) * vv);
+                acc += static_cast<float>(q[d]) * s[i];
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            acc[c] += __shfl_xor(acc[c], 16);
+            acc[c] += __shfl_xor(acc[c], 32);
+        }
+        if (lane < 16) *reinterpret_cast<f32x4 *>(&part[wave][4 * cx]) = acc;
+        __syncthreads();
+        if (tid < kStepCols && tile * kStepCols + tid < a.d2) {
+            T *o = static_cast<T *>(a.o) + b * a.os[0] + head * a.os[1] + tile * kStepCols + tid;
+            *o = static_cast<T>(a.scale * ((part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid])));
+        }
+        if (!again) break;
+        __syncthreads();
+        for (++b; b < a.batch; ++b)
+            if (a.slots[b] == slot) break;
+        if (b >= a.batch) break;
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int d = ry + 16 * i;
+        if (d < a.d1) {
+            if (a.vec) {
+                if (n0 < a.d2) *reinterpret_cast<f32x4 *>(state + static_cast<size_t>(d) * a.d2) = s[i];
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (n0 + c < a.d2) state[static_cast<size_t>(d) * a.d2 + c] = s[i][c];
+            }
+        }
+    }
+}
+
+template <typename T>
+int launch_step(const StepArgs &a, hipStream_t s) {
+    const unsigned blocks = static_cast<unsigned>(static_cast<size_t>(a.batch) * a.heads * ((a.d2 + kStepCols - 1) / kStepCols));
+    if (a.d1 <= 64) step_kernel<T, 4><<<blocks, 256, 0, s>>>(a);
+    else if (a.d1 <= 128) step_kernel<T, 8><<<blocks, 256, 0, s>>>(a);
+    else step_kernel<T, 16><<<blocks, 256, 0, s>>>(a);
+    return check_launch("step_kernel");
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------
+
+typedef dsp_gpu_linear_attention_shape Shape;
+
+size_t sample_bytes(int type) { return type == DSP_GPU_F32 ? 4 : 2; }
+
+struct Range {
+    const char *p;
+    size_t bytes;
+};
+bool meet(const Range &a, const Range &b) { return a.p && b.p && a.bytes && b.bytes && a.p < b.p + b.bytes && b.p < a.p + a.bytes; }
+
+// bytes from the first to the last element of a strided [batch][n][heads][dim] array
+size_t extent(const long long *stride, size_t batch, size_t n, size_t heads, size_t dim, size_t size) {
+    return ((batch - 1) * stride[0] + (n - 1) * stride[1] + (heads - 1) * stride[2] + dim) * size;
+}
+
+int check_heads(const char *who, int heads, int heads_q, int heads_k, int heads_v, int dim_k, int dim_v, int type) {
+    if (type != DSP_GPU_F32 && type != DSP_GPU_F16 && type != DSP_GPU_BF16) return fail(DSP_GPU_EINVAL, "%s: sample type %d (F32, F16 or BF16)", who, type);
+    if (heads < 1 || heads > kMaxHeads) return fail(DSP_GPU_EINVAL, "%s: %d heads outside [1,%d]", who, heads, kMaxHeads);
+    for (int h : {heads_q, heads_k, heads_v})
+        if (h < 1 || heads % h) return fail(DSP_GPU_EINVAL, "%s: %d heads of q, k or v do not divide %d", who, h, heads);
+    if (dim_k < 1 || dim_k > 256 || dim_v < 1 || dim_v > 256)
+        return fail(DSP_GPU_EINVAL, "%s: dimensions %d, %d outside [1,256]", who, dim_k, dim_v);
+    return DSP_GPU_OK;
+}
+
+int check_decay(const char *who, const double *log_decay, int heads, double scale, float *log2_decay) {
+    for (int h = 0; h < heads; ++h) {
+        if (!(log_decay[h] <= 0.0)) return fail(DSP_GPU_EINVAL, "%s: log_decay[%d] = %g is not <= 0", who, h, log_decay[h]);
+        log2_decay[h] = static_cast<float>(log_decay[h] * 1.4426950408889634);
+    }
+    if (!std::isfinite(scale)) return fail(DSP_GPU_EINVAL, "%s: non-finite scale", who);
+    return DSP_GPU_OK;
+}
+
+int check_shape(const char *who, const Shape &p) {
+    if (int rc = check_heads(who, p.heads, p.heads_q, p.heads_k, p.heads_v, p.dim_k, p.dim_v, p.sample_type)) return rc;
+    if (p.offsets && p.lengths) return fail(DSP_GPU_EINVAL, "%s: offsets and lengths exclude each other", who);
+    if (p.batch > (1u << 24) || p.n > (1ull << 31) || p.rows > (1ull << 31)) return fail(DSP_GPU_EINVAL, "%s: too many sequences or tokens", who);
+    for (const long long *s : {p.q_stride, p.k_stride, p.v_stride, p.o_stride})
+        for (int i = 0; i < 3; ++i)
+            if (s[i] < 0 || s[i] > (1ll << 40)) return fail(DSP_GPU_EINVAL, "%s: stride %lld", who, s[i]);
+    return DSP_GPU_OK;
+}
+
+// One launch of the kernel: up to three roles that share the padded first dimension and the columns of a workgroup.
+struct Plan {
+    int d1p, nt, segments;
+    long long seg_len;
+};
+
+constexpr size_t kFill = 512;  // workgroups that fill the chip: two on each of 256 CUs
+
+// How the work of `roles` runs over batch * heads sequences is spread.  A workgroup that owns 128 columns reads q and k half
+// as often as two that own 64, so columns are split only to fill the chip; then the time axis is cut into segments, which
+// costs a second pass over k and v, so the segments stay as few and as long as the chip allows.
+Plan make_plan(const Shape &p, int d1, const int *d2, int roles) {
+    Plan pl{};
+    pl.d1p = d1 <= 64 ? 64 : d1 <= 128 ? 128 : 256;
+    const size_t runs = p.batch * static_cast<size_t>(p.heads);
+    auto groups = [&](int nt) {
+        size_t t = 0;
+        for (int r = 0; r < roles; ++r) t += (d2[r] + 64 * nt - 1) / (64 * nt);
+        return runs * t;
+    };
+    bool wide = false;
+    for (int r = 0; r < roles; ++r) wide = wide || d2[r] > 64;
+    pl.nt = pl.d1p < 256 && wide ? 2 : 1;
+    const size_t w = groups(pl.nt);
+    const long long n = static_cast<long long>(p.offsets ? std::min(p.n, p.rows) : p.n), chunk = 64;
+    pl.segments = 1;
+    pl.seg_len = (n + chunk - 1) / chunk * chunk;
+    if (w < kFill / 2 && n >= 8 * chunk) {
+        const long long want = std::min<long long>(static_cast<long long>((kFill + w - 1) / w), n / (4 * chunk));
+        pl.seg_len = ((n + want - 1) / want + chunk - 1) / chunk * chunk;
+        pl.segments = static_cast<int>((n + pl.seg_len - 1) / pl.seg_len);
+    }
+    return pl;
+}
+
+size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+
+size_t segment_bytes(const Shape &p, const Plan &pl) {
+    return pl.segments > 1 ? align256(sizeof(float) * p.batch * p.heads * pl.segments * p.dim_k * p.dim_v) : 0;
+}
+size_t total_rows(const Shape &p) { return p.offsets ? p.rows : p.batch * p.n; }
+size_t part_bytes(const Shape &p, int heads_x, int dim) {
+    return heads_x < p.heads ? align256(sizeof(float) * total_rows(p) * p.heads * dim) : 0;
+}
+
+int launch_kernel(const Args &a, const Plan &pl, int type, unsigned blocks, bool state_only, hipStream_t s) {
+    if (type == DSP_GPU_BF16) return launch_bf16(a, pl.d1p, pl.nt, blocks, state_only, s);
+    if (type == DSP_GPU_F16) return launch_f16(a, pl.d1p, pl.nt, blocks, state_only, s);
+    return launch_f32(a, pl.d1p, pl.nt, blocks, state_only, s);
+}
+
+// roles: a.role[0 .. a.roles) with everything but tiles and seg filled in; seg_ws: a.roles * segment_bytes
+int run(const Shape &p, Args &a, const Plan &pl, char *seg_ws, hipStream_t s) {
+    a.heads = p.heads;
+    a.batch = static_cast<int>(p.batch);
+    a.n = static_cast<long long>(p.n);
+    a.rows = static_cast<long long>(p.rows);
+    a.offsets = p.offsets;
+    a.lengths = p.lengths;
+    a.segments = pl.segments;
+    a.seg_len = pl.seg_len;
+    size_t tiles = 0, most = 0;
+    bool ends = false;
+    for (int r = 0; r < a.roles; ++r) {
+        Role &x = a.role[r];
+        x.tiles = (x.d2 + 64 * pl.nt - 1) / (64 * pl.nt);
+        x.seg = pl.segments > 1 ? reinterpret_cast<float *>(seg_ws + r * segment_bytes(p, pl)) : nullptr;
+        tiles += x.tiles;
+        most = std::max<size_t>(most, (static_cast<size_t>(x.d1) * x.d2 + 255) / 256);
+        ends = ends || x.s_out;
+    }
+    const size_t runs = p.batch * p.heads, blocks = runs * tiles * pl.segments;
+    if (blocks > 0x7fffffffu || runs * most > 0x7fffffffu) return fail(DSP_GPU_EINVAL, "linear attention: %zu workgroups", blocks);
+    if (pl.segments > 1) {
+        if (int rc = launch_kernel(a, pl, p.sample_type, static_cast<unsigned>(runs * tiles * (pl.segments - (ends ? 0 : 1))), true, s)) return rc;
+        join_segments_kernel<<<dim3(static_cast<unsigned>(runs * most), a.roles), 256, 0, s>>>(a);
+        if (int rc = check_launch("join_segments_kernel")) return rc;
+    }
+    return launch_kernel(a, pl, p.sample_type, static_cast<unsigned>(blocks), false, s);
+}
+
+void set_strides(long long *to, const long long *from) {
+    for (int i = 0; i < 3; ++i) to[i] = from[i];
+}
+
+// 16-byte accesses of a tensor: whole packs in a row, and every row aligned
+bool packs(const void *p, const long long *stride, int dim, int type) {
+    const long long ve = type == DSP_GPU_BF16 ? 8 : 4;
+    const size_t align = ve * sample_bytes(type);
+    return reinterpret_cast<uintptr_t>(p) % align == 0 && dim % ve == 0 && stride[0] % ve == 0 && stride[1] % ve == 0 && stride[2] % ve == 0;
+}
+bool quads(const void *p, const long long *stride, int dim, size_t size) {
+    return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && dim % 4 == 0 && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[2] % 4 == 0;
+}
+
+struct Tensor {
+    const void *p;
+    const long long *stride;
+    int heads, dim;
+};
+
+void fill_role(Role &r, const Shape &p, const Tensor &q, const Tensor &k, const Tensor &v, void *o, const long long *o_stride, bool partial) {
+    r.q = q.p, r.k = k.p, r.v = v.p, r.o = o;
+    set_strides(r.qs, q.stride), set_strides(r.ks, k.stride), set_strides(r.vs, v.stride), set_strides(r.os, o_stride);
+    r.q_group = p.heads / q.heads, r.k_group = p.heads / k.heads, r.v_group = p.heads / v.heads;
+    r.d1 = q.dim, r.d2 = v.dim;
+    r.o_partial = partial;
+    r.vec = packs(q.p, q.stride, q.dim, p.sample_type) | packs(k.p, k.stride, k.dim, p.sample_type) << 1 |
+            packs(v.p, v.stride, v.dim, p.sample_type) << 2 | quads(o, o_stride, v.dim, partial ? 4 : sample_bytes(p.sample_type)) << 3;
+}
+
+struct BackwardPlan {
+    Plan pl[3];     // of dq, dk, dv
+    int launches;   // 1: the three in one launch (pl[0]); 2: dq and dk in one, dv in another
+    size_t seg, part[3], total;
+};
+
+BackwardPlan backward_plan(const Shape &p) {
+    BackwardPlan bp{};
+    auto pad = [](int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; };
+    const int d2[3] = {p.dim_k, p.dim_k, p.dim_v};
+    if (pad(p.dim_k) == pad(p.dim_v)) {
+        bp.launches = 1;
+        bp.pl[0] = make_plan(p, p.dim_k, d2, 3);
+        bp.seg = 3 * segment_bytes(p, bp.pl[0]);
+    } else {  // the launches follow one another: the segments of the second take the place of the first's
+        bp.launches = 2;
+        bp.pl[0] = make_plan(p, p.dim_v, d2, 2);
+        bp.pl[2] = make_plan(p, p.dim_k, d2 + 2, 1);
+        bp.seg = std::max(2 * segment_bytes(p, bp.pl[0]), segment_bytes(p, bp.pl[2]));
+    }
+    bp.part[0] = part_bytes(p, p.heads_q, p.dim_k);
+    bp.part[1] = part_bytes(p, p.heads_k, p.dim_k);
+    bp.part[2] = part_bytes(p, p.heads_v, p.dim_v);
+    bp.total = bp.seg + bp.part[0] + bp.part[1] + bp.part[2];
+    return bp;
+}
+
+int take_workspace(const char *who, size_t need, void *given, size_t given_bytes, hipStream_t s, char **out) {
+    *out = nullptr;
+    if (need == 0) return DSP_GPU_OK;
+    if (given) {
+        if (given_bytes < need) return fail(DSP_GPU_EINVAL, "%s: a workspace of %zu bytes, %zu are needed", who, given_bytes, need);
+        if (reinterpret_cast<uintptr_t>(given) % 16) return fail(DSP_GPU_EINVAL, "%s: workspace not aligned to 16 bytes", who);
+        *out = static_cast<char *>(given);
+        return DSP_GPU_OK;
+    }
+    void *p = nullptr;
+    if (int rc = workspace(WS_ATTENTION, need, &p, s)) return rc;
+    *out = static_cast<char *>(p);
+    return DSP_GPU_OK;
+}
+
+template <typename T>
+int add_heads(const Args &a, const Shape &p, const float *part, void *out, int heads_x, int dim, hipStream_t s) {
+    add_heads_kernel<T><<<static_cast<unsigned>(total_rows(p)), 256, 0, s>>>(a, part, static_cast<T *>(out), p.heads / heads_x, dim);
+    return check_launch("add_heads_kernel");
+}
+
+size_t state_bytes(const Shape &p) { return sizeof(float) * p.batch * p.heads * p.dim_k * p.dim_v; }
+
+}  // namespace
+}  // namespace la
+}  // namespace dspgpu
+
+using namespace dspgpu;
+using namespace dspgpu::la;
+
+extern "C" {
+
+int dsp_gpu_linear_attention_workspace(const dsp_gpu_linear_attention_shape *shape, int backward, size_t *bytes) {
+    static const char *who = "dsp_gpu_linear_attention_workspace";
+    if (!shape || !bytes) return fail(DSP_GPU_EINVAL, "%s: null argument", who);
+    if (int rc = check_shape(who, *shape)) return rc;
+    *bytes = 0;
+    if (shape->batch == 0 || shape->n == 0 || (shape->offsets && shape->rows == 0)) return DSP_GPU_OK;
+    if (backward) {
+        *bytes = backward_plan(*shape).total;
+    } else {
+        const Plan pl = make_plan(*shape, shape->dim_k, &shape->dim_v, 1);
+        *bytes = segment_bytes(*shape, pl);
+    }
+    return DSP_GPU_OK;
+}
+
+int dsp_gpu_linear_attention(const void *q, const void *k, const void *v, void *o, const dsp_gpu_linear_attention_shape *shape,
+                             const double *log_decay, double scale, const float *state_in, float *state_out, void *workspace,
+                             size_t workspace_bytes, void *stream) {
+    static const char *who = "dsp_gpu_linear_attention";
+    if (!shape || !log_decay) return fail(DSP_GPU_EINVAL, "%s: null argument", who);
+    const Shape &p = *shape;
+    if (int rc = check_shape(who, p)) return rc;
+    Args a{};
+    if (int rc = check_decay(who, log_decay, p.heads, scale, a.log2_decay)) return rc;
+    if (p.batch == 0) return DSP_GPU_OK;
+    const size_t rows = total_rows(p);
+    if (rows && p.n && (!q || !k || !v || !o)) return fail(DSP_GPU_EINVAL, "%s: null buffer", who);
+    const size_t size = sample_bytes(p.sample_type), sb = state_bytes(p);
+    if (rows && p.n) {
+        const size_t batch = p.offsets ? 1 : p.batch, n = p.offsets ? p.rows : p.n;
+        if (!rows_distinct(p.o_stride, batch, n, p.heads, p.dim_v)) return fail(DSP_GPU_EINVAL, "%s: rows of o overlap one another", who);
+        const Range ro{static_cast<const char *>(o), extent(p.o_stride, batch, n, p.heads, p.dim_v, size)};
+        const Range rs_in{reinterpret_cast<const char *>(state_in), sb}, rs_out{reinterpret_cast<const char *>(state_out), sb};
+        for (const Range &x : {Range{static_cast<const char *>(q), extent(p.q_stride, batch, n, p.heads_q, p.dim_k, size)},
+                               Range{static_cast<const char *>(k), extent(p.k_stride, batch, n, p.heads_k, p.dim_k, size)},
+                               Range{static_cast<const char *>(v), extent(p.v_stride, batch, n, p.heads_v, p.dim_v, size)}})
+            if (meet(x, ro) || meet(x, rs_out)) return fail(DSP_GPU_EINVAL, "%s: an output overlaps q, k or v", who);
+        if (meet(ro, rs_in) || meet(ro, rs_out)) return fail(DSP_GPU_EINVAL, "%s: o overlaps a state", who);
+    }
+    if (state_in != state_out && meet({reinterpret_cast<const char *>(state_in), sb}, {reinterpret_cast<const char *>(state_out), sb}))
+        return fail(DSP_GPU_EINVAL, "%s: the states overlap", who);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const Plan pl = make_plan(p, p.dim_k, &p.dim_v, 1);
+    char *ws = nullptr;
+    if (int rc = take_workspace(who, rows && p.n ? segment_bytes(p, pl) : 0, workspace, workspace_bytes, s, &ws)) return rc;
+    a.roles = 1;
+    Role &r = a.role[0];
+    fill_role(r, p, {q, p.q_stride, p.heads_q, p.dim_k}, {k, p.k_stride, p.heads_k, p.dim_k}, {v, p.v_stride, p.heads_v, p.dim_v}, o, p.o_stride, false);
+    r.read = r.pscale = static_cast<float>(scale);
+    r.write = 1.0f;
+    r.s_in = state_in;
+    r.s_in_d = p.dim_v;
+    r.s_in_n = 1;
+    r.s_out = state_out;
+    if (int rc = run(p, a, pl, ws, s)) return rc;
+    if (!p.zero_rest || !(p.offsets || p.lengths) || !rows || !p.n) return DSP_GPU_OK;
+    Rest z{};
+    z.p[0] = o;
+    set_strides(z.stride[0], p.o_stride);
+    z.heads[0] = p.heads;
+    z.dim[0] = p.dim_v;
+    z.wide = size == 4;
+    z.rows = static_cast<long long>(rows);
+    return zero_rest(a, z, 1, s);
+}
+
+int dsp_gpu_linear_attention_backward(const void *q, const void *k, const void *v, const void *dout, void *dq, void *dk, void *dv,
+                                      const dsp_gpu_linear_attention_shape *shape, const double *log_decay, double scale,
+                                      const float *state_in, const float *dstate_out, float *dstate_in, void *workspace,
+                                      size_t workspace_bytes, void *stream) {
+    static const char *who = "dsp_gpu_linear_attention_backward";
+    if (!shape || !log_decay) return fail(DSP_GPU_EINVAL, "%s: null argument", who);
+    const Shape &p = *shape;
+    if (int rc = check_shape(who, p)) return rc;
+    Args a{};
+    if (int rc = check_decay(who, log_decay, p.heads, scale, a.log2_decay)) return rc;
+    if (p.batch == 0) return DSP_GPU_OK;
+    const size_t rows = total_rows(p), size = sample_bytes(p.sample_type), sb = state_bytes(p);
+    if (rows && p.n && (!q || !k || !v || !dout || !dq || !dk || !dv)) return fail(DSP_GPU_EINVAL, "%s: null buffer", who);
+    if (rows > 0x7fffffffu) return fail(DSP_GPU_EINVAL, "%s: %zu rows", who, rows);
+    if (rows && p.n) {
+        const size_t batch = p.offsets ? 1 : p.batch, n = p.offsets ? p.rows : p.n;
+        const Range out[4] = {{static_cast<const char *>(dq), rows * p.heads_q * p.dim_k * size},
+                              {static_cast<const char *>(dk), rows * p.heads_k * p.dim_k * size},
+                              {static_cast<const char *>(dv), rows * p.heads_v * p.dim_v * size},
+                              {reinterpret_cast<const char *>(dstate_in), sb}};
+        const Range in[5] = {{static_cast<const char *>(q), extent(p.q_stride, batch, n, p.heads_q, p.dim_k, size)},
+                             {static_cast<const char *>(k), extent(p.k_stride, batch, n, p.heads_k, p.dim_k, size)},
+                             {static_cast<const char *>(v), extent(p.v_stride, batch, n, p.heads_v, p.dim_v, size)},
+                             {static_cast<const char *>(dout), extent(p.o_stride, batch, n, p.heads, p.dim_v, size)},
+                             {reinterpret_cast<const char *>(state_in), sb}};
+        for (int i = 0; i < 4; ++i) {
+            for (const Range &x : in)
+                if (meet(out[i], x)) return fail(DSP_GPU_EINVAL, "%s: a gradient overlaps an input", who);
+            for (int j = 0; j < i; ++j)
+                if (meet(out[i], out[j])) return fail(DSP_GPU_EINVAL, "%s: two gradients overlap", who);
+        }
+    }
+    // dk reads dstate_out while dv writes dstate_in: not in place
+    if (meet({reinterpret_cast<const char *>(dstate_in), sb}, {reinterpret_cast<const char *>(dstate_out), sb}))
+        return fail(DSP_GPU_EINVAL, "%s: dstate_in and dstate_out overlap", who);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const BackwardPlan bp = backward_plan(p);
+    char *ws = nullptr;
+    if (int rc = take_workspace(who, rows && p.n ? bp.total : 0, workspace, workspace_bytes, s, &ws)) return rc;
+
+    const Tensor tq{q, p.q_stride, p.heads_q, p.dim_k}, tk{k, p.k_stride, p.heads_k, p.dim_k}, tv{v, p.v_stride, p.heads_v, p.dim_v},
+        tdo{dout, p.o_stride, p.heads, p.dim_v};
+    void *grad[3] = {dq, dk, dv};
+    const int heads_x[3] = {p.heads_q, p.heads_k, p.heads_v}, dim[3] = {p.dim_k, p.dim_k, p.dim_v};
+    float *part[3];
+    Role role[3] = {};
+    char *at = ws + bp.seg;
+    for (int i = 0; i < 3; ++i) {
+        part[i] = bp.part[i] ? reinterpret_cast<float *>(at) : nullptr;
+        at += bp.part[i];
+        const long long h = part[i] ? p.heads : heads_x[i];
+        const long long st[3] = {static_cast<long long>(p.n) * h * dim[i], h * dim[i], dim[i]};
+        const Tensor &x = i == 0 ? tdo : i == 1 ? tv : tk, &y = i == 0 ? tv : i == 1 ? tdo : tq, &z = i == 0 ? tk : i == 1 ? tq : tdo;
+        fill_role(role[i], p, x, y, z, part[i] ? part[i] : grad[i], st, part[i] != nullptr);
+        const float sc = static_cast<float>(scale);
+        role[i].pscale = sc;
+        role[i].read = i == 0 ? sc : 1.0f;
+        role[i].write = i == 0 ? 1.0f : sc;
+        role[i].late = i != 0;
+        role[i].s_in = i == 0 ? state_in : dstate_out;
+        role[i].s_in_d = i == 2 ? p.dim_v : 1;  // the states of dq and dk are S^T and dS^T
+        role[i].s_in_n = i == 2 ? 1 : p.dim_v;
+        role[i].s_out = i == 2 ? dstate_in : nullptr;
+    }
+    if (bp.launches == 1) {
+        a.roles = 3;
+        for (int i = 0; i < 3; ++i) a.role[i] = role[i];
+        if (int rc = run(p, a, bp.pl[0], ws, s)) return rc;
+    } else {
+        a.roles = 2;
+        a.role[0] = role[0];
+        a.role[1] = role[1];
+        if (int rc = run(p, a, bp.pl[0], ws, s)) return rc;
+        a.roles = 1;
+        a.role[0] = role[2];
+        if (int rc = run(p, a, bp.pl[2], ws, s)) return rc;
+    }
+    for (int i = 0; i < 3; ++i) {
+        if (!part[i] || !rows || !p.n) continue;
+        int rc = p.sample_type == DSP_GPU_BF16 ? add_heads<__bf16>(a, p, part[i], grad[i], heads_x[i], dim[i], s)
+                 : p.sample_type == DSP_GPU_F16 ? add_heads<_Float16>(a, p, part[i], grad[i], heads_x[i], dim[i], s)
+                                                : add_heads<float>(a, p, part[i], grad[i], heads_x[i], dim[i], s);
+        if (rc) return rc;
+    }
+    if (!p.zero_rest || !(p.offsets || p.lengths) || !rows || !p.n) return DSP_GPU_OK;
+    Rest z{};
+    for (int i = 0; i < 3; ++i) {
+        z.p[i] = grad[i];
+        z.heads[i] = heads_x[i];
+        z.dim[i] = dim[i];
+        z.stride[i][2] = dim[i];
+        z.stride[i][1] = z.stride[i][2] * heads_x[i];
+        z.stride[i][0] = z.stride[i][1] * static_cast<long long>(p.n);
+    }
+    z.wide = size == 4;
+    z.rows = static_cast<long long>(rows);
+    return zero_rest(a, z, 3, s);
+}
+
+int dsp_gpu_linear_attention_step(const void *q, const void *k, const void *v, void *o, const dsp_gpu_linear_attention_shape *shape,
+                                  const double *log_decay, double scale, float *state, const long long *slots, size_t n_slots,
+                                  void *stream) {
+    static const char *who = "dsp_gpu_linear_attention_step";
+    if (!shape || !log_decay) return fail(DSP_GPU_EINVAL, "%s: null argument", who);
+    const Shape &p = *shape;
+    if (int rc = check_shape(who, p)) return rc;
+    StepArgs a{};
+    if (int rc = check_decay(who, log_decay, p.heads, scale, a.decay_hi)) return rc;
+    for (int h = 0; h < p.heads; ++h) {
+        const double w = std::exp(log_decay[h]);
+        a.decay_hi[h] = static_cast<float>(w);
+        a.decay_lo[h] = static_cast<float>(w - a.decay_hi[h]);
+    }
+    if (p.n != 1 || p.offsets || p.lengths) return fail(DSP_GPU_EINVAL, "%s: one token a row (n = 1), no offsets or lengths", who);
+    if (p.batch == 0) return DSP_GPU_OK;
+    if (!q || !k || !v || !o || !state) return fail(DSP_GPU_EINVAL, "%s: null buffer", who);
+    const size_t states = slots ? n_slots : p.batch, size = sample_bytes(p.sample_type);
+    if (states == 0 || states > (1ull << 31)) return fail(DSP_GPU_EINVAL, "%s: %zu slots", who, states);
+    if (!rows_distinct(p.o_stride, p.batch, 1, p.heads, p.dim_v)) return fail(DSP_GPU_EINVAL, "%s: rows of o overlap one another", who);
+    const Range rs{reinterpret_cast<const char *>(state), sizeof(float) * states * p.heads * p.dim_k * p.dim_v};
+    const Range ro{static_cast<const char *>(o), extent(p.o_stride, p.batch, 1, p.heads, p.dim_v, size)};
+    for (const Range &x : {Range{static_cast<const char *>(q), extent(p.q_stride, p.batch, 1, p.heads_q, p.dim_k, size)},
+                           Range{static_cast<const char *>(k), extent(p.k_stride, p.batch, 1, p.heads_k, p.dim_k, size)},
+                           Range{static_cast<const char *>(v), extent(p.v_stride, p.batch, 1, p.heads_v, p.dim_v, size)},
+                           Range{reinterpret_cast<const char *>(slots), slots ? sizeof(long long) * p.batch : 0}})
+        if (meet(x, ro) || meet(x, rs)) return fail(DSP_GPU_EINVAL, "%s: o or the state overlaps an input", who);
+    if (meet(ro, rs)) return fail(DSP_GPU_EINVAL, "%s: o overlaps the state", who);
+    const size_t blocks = p.batch * p.heads * ((p.dim_v + kStepCols - 1) / kStepCols);
+    if (blocks > 0x7fffffffu) return fail(DSP_GPU_EINVAL, "%s: %zu workgroups", who, blocks);
+    a.q = q, a.k = k, a.v = v, a.o = o;
+    a.qs[0] = p.q_stride[0], a.qs[1] = p.q_stride[2];
+    a.ks[0] = p.k_stride[0], a.ks[1] = p.k_stride[2];
+    a.vs[0] = p.v_stride[0], a.vs[1] = p.v_stride[2];
+    a.os[0] = p.o_stride[0], a.os[1] = p.o_stride[2];
+    a.q_group = p.heads / p.heads_q, a.k_group = p.heads / p.heads_k, a.v_group = p.heads / p.heads_v;
+    a.heads = p.heads, a.d1 = p.dim_k, a.d2 = p.dim_v;
+    a.batch = static_cast<int>(p.batch);
+    a.scale = static_cast<float>(scale);
+    a.vec = p.dim_v % 4 == 0 && reinterpret_cast<uintptr_t>(state) % 16 == 0;
+    a.state = state;
+    a.slots = slots;
+    a.n_slots = static_cast<long long>(n_slots);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (p.sample_type == DSP_GPU_BF16) return launch_step<__bf16>(a, s);
+    if (p.sample_type == DSP_GPU_F16) return launch_step<_Float16>(a, s);
+    return launch_step<float>(a, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,12 @@
+// linear_attention_f32.hip -- the kernels of linear_attention_core.h for one sample type.
+#include "linear_attention_core.h"
+
+namespace dspgpu {
+namespace la {
+
+int launch_f32(const Args &a, int d1p, int nt, unsigned blocks, bool state_only, hipStream_t s) {
+    return launch_any<float, float>(a, d1p, nt, blocks, state_only, s);
+}
+
+}  // namespace la
+}  // namespace dspgpu

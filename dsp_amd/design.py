@@ -186,3 +186,46 @@ def peaking(f: float, gain_db: float, q: float):
     z = (.5 + y) * math.cos(f)
     a0 = .5 - y
     return np.array([a0, 0.0, -a0]), np.array([0.0, 2 * z, -2 * y]), u - 1, 1.0
+
+
+# ---- sequence layers (ops.rotary, ops.linear_attention) --------------------------------------------------------------------
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                       original_length: int = 4096, fast_turns: float = 32.0, slow_turns: float = 1.0) -> np.ndarray:
+    """Radians a position of the rot_dim/2 pairs of ops.rotary: base^(-2i/rot_dim), for contexts `factor` times longer by
+
+    "none"    as they are
+    "linear"  every frequency divided by factor (positions interpolated)
+    "base"    a larger base, such that the slowest pair is slowed by exactly factor and the fastest not at all
+    "ramp"    pairs that turn more than fast_turns times over original_length positions kept, those that turn less than
+              slow_turns times divided by factor, a linear mixture of both in between
+    """
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim {rot_dim} is not an even number >= 2")
+    if not (base > 0 and factor > 0):
+        raise ValueError("base and factor must be positive")
+    i = np.arange(rot_dim // 2, dtype=np.float64)
+    if scaling == "base":
+        if rot_dim > 2:
+            base = base * factor ** (rot_dim / (rot_dim - 2.0))
+        scaling = "none"
+    f = base ** (-2.0 * i / rot_dim)
+    if scaling == "none":
+        return f
+    if scaling == "linear":
+        return f / factor
+    if scaling == "ramp":
+        if not fast_turns > slow_turns:
+            raise ValueError("fast_turns must be greater than slow_turns")
+        turns = original_length * f / (2 * PI)
+        keep = np.clip((turns - slow_turns) / (fast_turns - slow_turns), 0.0, 1.0)
+        return f * (keep + (1.0 - keep) / factor)
+    raise ValueError(f"scaling {scaling!r}")
+
+
+def head_decays(heads: int, fastest: float = 1.0 / 32, slowest: float = 1.0 / 512) -> np.ndarray:
+    """log_decay of ops.linear_attention: ln(1 - r) with the rate r of the heads spread evenly in its logarithm from
+    `fastest` to `slowest` (a head of rate r remembers about 1/r tokens)."""
+    if heads < 1 or not (0 < slowest < 1 and 0 < fastest < 1):
+        raise ValueError("heads >= 1 and rates between 0 and 1 are needed")
+    r = np.exp(np.linspace(math.log(fastest), math.log(slowest), heads))
+    return np.log1p(-r)

@@ -8,8 +8,15 @@ Names and argument meaning follow the reference (file:line relative to its dsp/i
     moving_average(x, npoints)        filter.h:81-101
     iir(x, a, b, c0, d0, state, mode) coefficients.h:88-130,172-195
 
+Sequence layers (no counterpart in the reference; torch CUDA tensors, fp32, fp16 or bf16):
+
+    rotary(x, inv_freq, positions)                    pairs of each head turned by pos * inv_freq, and back
+    linear_attention(q, k, v, log_decay)              S_t = w S_{t-1} + k_t v_t^T, o_t = scale q_t S_t, whole sequences
+    linear_attention_backward(q, k, v, log_decay, do) its gradients
+    linear_attention_step(q, k, v, log_decay, state)  one token a row, states updated in place
+
 Inputs are torch CUDA tensors (device pointers, asynchronous on the current torch stream)
-or numpy arrays (host pointers, staged by the library).  fp32 only.  No CPU fallback.
+or numpy arrays (host pointers, staged by the library).  fp32 unless a name says otherwise.  No CPU fallback.
 """
 from __future__ import annotations
 
@@ -350,6 +357,212 @@ def biquad_swept(x, fc, bandwidth: float, kind: str = "bandpass", state=None, ou
         capi.check(capi.lib().dsp_gpu_biquad_swept(px, pfc, _ptr(y), channels, n, stride, _SWEPT_KINDS[kind],
                                                    float(bandwidth), pstate, mem, _stream_of(x)))
     return y
+
+
+# ---- sequence layers -------------------------------------------------------------------------------------------------
+
+
+def _bad(message):
+    return capi.DspGpuError(capi.EINVAL, message)
+
+
+def _sample_type(x, what):
+    if not _is_torch(x) or not x.is_cuda:
+        raise _bad(f"{what} must be a torch tensor on the GPU")
+    types = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
+    if x.dtype not in types:
+        raise _bad(f"{what}: expected float32, float16 or bfloat16, got {x.dtype}")
+    return types[x.dtype]
+
+
+def _strides(x, what, packed=False):
+    """(batch, token, head) strides of a [batch, n, heads, dim] (packed: [rows, heads, dim]) tensor; 0 for an axis of one."""
+    if x.shape[-1] > 1 and x.stride(-1) != 1 and x.numel():
+        raise _bad(f"{what}: the last axis must be contiguous")
+    st = [0 if n <= 1 else s for n, s in zip(x.shape[:-1], x.stride()[:-1])]
+    return [0] + st if packed else st
+
+
+def _index(x, like, count, what):
+    """A device int64 array of `count` entries."""
+    if not (_is_torch(x) and x.device == like.device and x.dtype == torch.int64 and tuple(x.shape) == (count,)
+            and x.is_contiguous()):
+        raise _bad(f"{what} must be a contiguous int64 tensor of {count} entries on x's device")
+    return x.data_ptr() if count else None
+
+
+def rotary(x, inv_freq, positions=None, position: int = 0, layout: str = "half", inverse: bool = False, gain: float = 1.0,
+           out=None):
+    """Rotary positions (dsp_gpu_rotary).  x [batch, n, heads, dim] or [n, heads, dim], any strides with a contiguous last
+    axis; the first 2 * len(inv_freq) elements of each head are turned by the angle pos * inv_freq (host doubles,
+    design.rotary_frequencies), pairs (i, i + half) for layout "half", (2i, 2i + 1) for "interleaved"; the rest is copied.
+    positions: int64 [batch, n] or [n] on x's device, or None: position, position + 1, ...  inverse: the other way round --
+    the gradient of the forward call, with the same gain.  out may be x (in place) or any tensor of its shape."""
+    kind = _sample_type(x, "x")
+    if x.ndim not in (3, 4):
+        raise _bad("x must be [batch, n, heads, dim] or [n, heads, dim]")
+    layouts = {"half": capi.ROTARY_HALF, "interleaved": capi.ROTARY_INTERLEAVED}
+    if layout not in layouts:
+        raise _bad(f"layout {layout!r}")
+    inv_freq = np.ascontiguousarray(inv_freq, dtype=np.float64)
+    if inv_freq.ndim != 1:
+        raise _bad("inv_freq must be one-dimensional")
+    y = torch.empty_like(x, memory_format=torch.contiguous_format) if out is None else out
+    if not _is_torch(y) or y.device != x.device or y.dtype != x.dtype or y.shape != x.shape:
+        raise _bad("out must have x's shape and type, on x's device")
+    x4, y4 = (x, y) if x.ndim == 4 else (x[None], y[None])
+    batch, n, heads, dim = x4.shape
+    ppos = pstride = None
+    if positions is not None:
+        if not (_is_torch(positions) and positions.device == x.device and positions.dtype == torch.int64
+                and tuple(positions.shape) in ((batch, n), (n,))):
+            raise _bad("positions must be int64 [batch, n] or [n] on x's device")
+        p2 = positions.expand(batch, n)
+        pstride = (C.c_longlong * 2)(*[0 if c <= 1 else s for c, s in zip(p2.shape, p2.stride())])
+        ppos = positions.data_ptr() if x.numel() else None
+    xs, ys = (C.c_longlong * 3)(*_strides(x4, "x")), (C.c_longlong * 3)(*_strides(y4, "out"))
+    with _on_device(x):
+        capi.check(capi.lib().dsp_gpu_rotary(x.data_ptr(), y.data_ptr(), kind, batch, n, heads, dim, xs, ys,
+                                             inv_freq.ctypes.data, 2 * inv_freq.size, layouts[layout], ppos, pstride,
+                                             int(position), float(gain), capi.INVERSE if inverse else capi.FORWARD,
+                                             _stream_of(x)))
+    return y
+
+
+def _attention_shape(q, k, v, log_decay, lengths, offsets, max_length, step=False):
+    """-> (shape, packed, log_decay, state shape); checks everything the C call cannot see."""
+    kind = _sample_type(q, "q")
+    for t, what in ((k, "k"), (v, "v")):
+        if _sample_type(t, what) != kind or t.device != q.device:
+            raise _bad(f"{what} must have q's type and device")
+    packed = offsets is not None
+    axes = 3 if packed or step else 4
+    if not (q.ndim == k.ndim == v.ndim == axes):
+        raise _bad("q, k and v must be " + ("[batch, heads, dim]" if step else "[rows, heads, dim] with offsets"
+                                            if packed else "[batch, n, heads, dim]"))
+    lead = q.shape[:axes - 2]
+    if k.shape[:axes - 2] != lead or v.shape[:axes - 2] != lead or k.shape[-1] != q.shape[-1]:
+        raise _bad(f"shapes of q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not belong together")
+    log_decay = np.ascontiguousarray(log_decay, dtype=np.float64)
+    if log_decay.ndim != 1:
+        raise _bad("log_decay must be one-dimensional: one value a head")
+    p = capi.LinearAttentionShape()
+    p.heads, p.heads_q, p.heads_k, p.heads_v = log_decay.size, q.shape[-2], k.shape[-2], v.shape[-2]
+    p.dim_k, p.dim_v, p.sample_type = q.shape[-1], v.shape[-1], kind
+    if packed:
+        if lengths is not None:
+            raise _bad("offsets and lengths exclude each other")
+        if offsets.ndim != 1 or offsets.numel() < 1:
+            raise _bad("offsets must have batch + 1 entries")
+        p.batch, p.rows = offsets.numel() - 1, lead[0]
+        p.n = lead[0] if max_length is None else int(max_length)
+        p.offsets = _index(offsets, q, p.batch + 1, "offsets")
+    elif step:
+        p.batch, p.n = lead[0], 1
+    else:
+        p.batch, p.n = lead
+        if lengths is not None:
+            p.lengths = _index(lengths, q, p.batch, "lengths")
+    if not packed and max_length is not None:
+        raise _bad("max_length goes with offsets")
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        st = _strides(t, name, packed)
+        getattr(p, name + "_stride")[:] = [st[0], 0, st[1]] if step else st
+    return p, packed, log_decay, (p.batch, p.heads, p.dim_k, p.dim_v)
+
+
+def _state(t, like, shape, what):
+    if t is None:
+        return None
+    if not (_is_torch(t) and t.device == like.device and t.dtype == torch.float32 and tuple(t.shape) == shape and t.is_contiguous()):
+        raise _bad(f"{what} must be a contiguous float32 tensor {shape} on q's device")
+    return t.data_ptr()
+
+
+def _attention_workspace(p, backward, like):
+    """A tensor of the bytes the call needs, or None: torch's allocator keeps calls, streams and captured graphs apart."""
+    need = C.c_size_t(0)
+    capi.check(capi.lib().dsp_gpu_linear_attention_workspace(C.byref(p), int(backward), C.byref(need)))
+    return torch.empty(need.value, dtype=torch.uint8, device=like.device) if need.value else None
+
+
+def _ws_args(ws):
+    return (None, 0) if ws is None else (ws.data_ptr(), ws.numel())
+
+
+def linear_attention(q, k, v, log_decay, scale: float = 1.0, state=None, new_state=None, lengths=None, offsets=None,
+                     max_length=None, out=None):
+    """Linear attention with a decay for each head (dsp_gpu_linear_attention): S_t = w S_{t-1} + k_t v_t^T and
+    o_t = scale * q_t S_t with w = exp(log_decay[head]).  q, k [batch, n, heads, dim_k], v [batch, n, heads, dim_v], heads
+    of each a divisor of len(log_decay); any strides with a contiguous last axis.  A packed batch: [rows, heads, dim] with
+    offsets int64 [batch + 1] on the device (max_length: the longest sequence, else all rows); a padded one: lengths int64
+    [batch].  state / new_state: float32 [batch, heads, dim_k, dim_v] before the first and after the last token (may be the
+    same tensor).  Returns o [batch, n, heads, dim_v] (rows of no sequence: zeros, or what `out` held)."""
+    p, packed, log_decay, st_shape = _attention_shape(q, k, v, log_decay, lengths, offsets, max_length)
+    shape = tuple(q.shape[:-2]) + (p.heads, p.dim_v)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        p.zero_rest = 1
+    elif not (_is_torch(out) and out.device == q.device and out.dtype == q.dtype and tuple(out.shape) == shape):
+        raise _bad(f"out must be a {q.dtype} tensor {shape} on q's device")
+    p.o_stride[:] = _strides(out, "out", packed)
+    s_in, s_out = _state(state, q, st_shape, "state"), _state(new_state, q, st_shape, "new_state")
+    with _on_device(q):
+        ws = _attention_workspace(p, False, q)
+        capi.check(capi.lib().dsp_gpu_linear_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), C.byref(p),
+                                                       log_decay.ctypes.data, float(scale), s_in, s_out, *_ws_args(ws),
+                                                       _stream_of(q)))
+    return out
+
+
+def linear_attention_backward(q, k, v, log_decay, dout, scale: float = 1.0, state=None, dnew_state=None, dstate=None,
+                              lengths=None, offsets=None, max_length=None):
+    """The gradients (dq, dk, dv) of linear_attention from dout and, where given, dnew_state, that of the state after the
+    last token.  `state`: as in the forward call.  dstate: a float32 tensor that receives the gradient of `state`.  Gradients
+    of heads that several share are summed in order; rows of no sequence get zeros.  log_decay has none."""
+    p, packed, log_decay, st_shape = _attention_shape(q, k, v, log_decay, lengths, offsets, max_length)
+    shape = tuple(q.shape[:-2]) + (p.heads, p.dim_v)
+    if not (_is_torch(dout) and dout.device == q.device and dout.dtype == q.dtype and tuple(dout.shape) == shape):
+        raise _bad(f"dout must be a {q.dtype} tensor {shape} on q's device")
+    p.o_stride[:] = _strides(dout, "dout", packed)
+    s_in, ds_out = _state(state, q, st_shape, "state"), _state(dnew_state, q, st_shape, "dnew_state")
+    ds_in = _state(dstate, q, st_shape, "dstate")
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
+    p.zero_rest = 1
+    with _on_device(q):
+        ws = _attention_workspace(p, True, q)
+        capi.check(capi.lib().dsp_gpu_linear_attention_backward(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), *(g.data_ptr() for g in grads), C.byref(p),
+            log_decay.ctypes.data, float(scale), s_in, ds_out, ds_in, *_ws_args(ws), _stream_of(q)))
+    return tuple(grads)
+
+
+def linear_attention_step(q, k, v, log_decay, state, scale: float = 1.0, slots=None, out=None):
+    """One token a row (dsp_gpu_linear_attention_step): q, k [batch, heads, dim_k], v [batch, heads, dim_v]; `state` float32
+    [batch, heads, dim_k, dim_v], updated in place -- or [n_slots, ...] with slots int64 [batch] on the device, row b working
+    on state[slots[b]] (a slot outside the pool: the row is skipped; the same slot twice: in the order of the rows).
+    Returns o [batch, heads, dim_v] (skipped rows: zeros)."""
+    p, _, log_decay, st_shape = _attention_shape(q, k, v, log_decay, None, None, None, step=True)
+    shape = (p.batch, p.heads, p.dim_v)
+    pslots, n_slots = None, 0
+    if slots is not None:
+        pslots = _index(slots, q, p.batch, "slots")
+        n_slots = state.shape[0] if _is_torch(state) and state.ndim else 0
+        st_shape = (n_slots,) + st_shape[1:]
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif not (_is_torch(out) and out.device == q.device and out.dtype == q.dtype and tuple(out.shape) == shape):
+        raise _bad(f"out must be a {q.dtype} tensor {shape} on q's device")
+    so = _strides(out, "out")
+    p.o_stride[:] = [so[0], 0, so[1]]
+    if state is None:
+        raise _bad("state must be given: it is what the step updates")
+    ps = _state(state, q, st_shape, "state")
+    with _on_device(q):
+        capi.check(capi.lib().dsp_gpu_linear_attention_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), C.byref(p),
+                                                            log_decay.ctypes.data, float(scale), ps, pslots, n_slots,
+                                                            _stream_of(q)))
+    return out
 
 
 def fft_kernel_ms(x, out, inverse: bool, iters: int) -> float:

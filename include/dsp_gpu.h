@@ -82,6 +82,9 @@ extern "C" {
 /* sample types of the entry points that take either (void pointers) */
 #define DSP_GPU_F32 0
 #define DSP_GPU_F64 1
+/* ... and of the sequence-layer entry points (dsp_gpu_rotary, dsp_gpu_linear_attention*): F32 or one of these */
+#define DSP_GPU_F16 2
+#define DSP_GPU_BF16 3
 
 /*
  * Batched complex FFT.  Replaces dsp::fft0<type>(in, out, log2n) (fft.h:31-55) for
@@ -270,6 +273,84 @@ int dsp_gpu_iir_multi_ex(const void *x, void *y, int sample_type, size_t channel
 #define DSP_GPU_SWEPT_BANDREJECT 1
 int dsp_gpu_biquad_swept(const float *x, const float *fc, float *y, size_t channels, size_t n, size_t fc_stride,
                          int kind, double bandwidth, double *state, int mem, void *stream);
+
+/*
+ * ---- Sequence layers ------------------------------------------------------------------------------------------------
+ * The recurrences and rotations that the token mixers of sequence models are made of.  NO COUNTERPART IN THE REFERENCE:
+ * one pole of dsp_gpu_iir per element of an outer product, and the rotation by e^{i pos f} that turns its real pole into a
+ * pair of complex ones.  DEVICE pointers only, asynchronous on `stream`, usable under graph capture; sample types F32, F16
+ * and BF16.  Tensors are [batch][n][heads][dim] in strides of ELEMENTS (batch, token, head; >= 0; the last axis is
+ * contiguous), so views of a fused projection are taken as they are.  log_decay and inv_freq are small HOST arrays, read
+ * during the call.
+ */
+
+/*
+ * Rotary positions.  For every token at position pos and every pair i of the first rot_dim elements of each head
+ *     (y0, y1) = gain * (x0 cos - x1 sin, x0 sin + x1 cos)      at the angle pos * inv_freq[i]
+ * pair i being elements (i, i + rot_dim/2) -- DSP_GPU_ROTARY_HALF -- or (2i, 2i+1) -- DSP_GPU_ROTARY_INTERLEAVED.  Elements
+ * from rot_dim on are copied.  DSP_GPU_INVERSE turns by the negative angle: the gradient of the forward call.  Angles are
+ * formed and reduced in double (positions of any size), cos and sin in fp32, the result rounded once.
+ * 2 <= rot_dim <= dim <= 1024, rot_dim even, rot_dim <= 256; inv_freq: rot_dim/2 finite doubles (radians a position;
+ * dsp_amd/design.py rotary_frequencies, also for long contexts).  positions: device int64, element (b, t) at
+ * b * position_stride[0] + t * position_stride[1] (strides >= 0, 0 = shared), or NULL: position + t.
+ * x == y with the same strides is in place; other overlaps are refused (DSP_GPU_EINVAL).  Gradients with respect to
+ * inv_freq and gain are not offered.
+ */
+#define DSP_GPU_ROTARY_HALF 0
+#define DSP_GPU_ROTARY_INTERLEAVED 1
+int dsp_gpu_rotary(const void *x, void *y, int sample_type, size_t batch, size_t n, int heads, int dim,
+                   const long long x_stride[3], const long long y_stride[3], const double *inv_freq, int rot_dim, int layout,
+                   const long long *positions, const long long position_stride[2], long long position, double gain,
+                   int direction, void *stream);
+
+/*
+ * Linear attention with a decay for each head.  With w = e^{log_decay[head]}, for every sequence and head
+ *     S_t = w S_{t-1} + k_t v_t^T          (S: [dim_k][dim_v], fp32)
+ *     o_t = scale * q_t S_t
+ * heads: how many states, decays and outputs a token has; q, k and v may have fewer heads (divisors of `heads`): head h
+ * reads head h / (heads / heads_q) of q, and so on.  1 <= heads <= 256, 1 <= dim_k, dim_v <= 256.
+ * log_decay: heads doubles <= 0 (-inf: nothing is remembered).  It is a constant of the head: no gradient is offered.
+ *   offsets   (device int64, batch + 1, may be NULL) a PACKED batch: sequence b is rows offsets[b] .. offsets[b+1] of
+ *             `rows` rows, the batch strides are not used and n is the length of the longest sequence
+ *   lengths   (device int64, batch, may be NULL) a PADDED batch: only the first lengths[b] tokens of sequence b are read
+ * Rows that belong to no sequence are not read, and not written either unless zero_rest asks for zeros there; values outside
+ * the tensors are taken as the nearest inside, and tokens from n on are left out.
+ *   state_in   [batch][heads][dim_k][dim_v] fp32, the state before the first token, or NULL: zero
+ *   state_out  the state after the last one (of an empty sequence: the one before), or NULL; may be state_in
+ * Forms a chunk of tokens at a time on the matrix cores, the state in fp32 registers; few long sequences are cut in time
+ * and joined.  bf16: products of bf16 operands (the weighted q k products and the state as read are rounded to bf16; what
+ * the state adds up is not); F16 and F32 multiply in fp32.  A NaN or infinity in a token's v reaches the tokens of its
+ * own chunk (up to 63 before it).  Outputs do not depend on anything but the inputs and the shape: repeated calls agree
+ * bit for bit.
+ * workspace: dsp_gpu_linear_attention_workspace bytes, 16-byte aligned, used until the call's work is done; NULL: the
+ * library's own per (device, stream), which grows -- not under capture, and not for two graphs that run at once.
+ *
+ * _backward: the gradients dq, dk, dv (contiguous, in the shapes of q, k, v, shared heads summed) from dout (o's shape and
+ * strides) and dstate_out (of state_out; NULL: zero); dstate_in (of state_in; may be NULL).  state_in as in the forward
+ * call.  Sums are ordered: no atomics.
+ *
+ * _step: one token a row (n = 1; token strides unused) on states updated in place.  state: [n_slots][heads][dim_k][dim_v],
+ * slots (device int64, batch): row b works on state slots[b]; a slot outside [0, n_slots) gives the row zeros for o and
+ * touches no state; rows that name the same slot take it in their order.  slots NULL: row b has state b, n_slots unused.
+ */
+typedef struct dsp_gpu_linear_attention_shape {
+    size_t batch, n, rows; /* rows: of a packed batch */
+    int heads, heads_q, heads_k, heads_v, dim_k, dim_v, sample_type;
+    long long q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+    const long long *offsets, *lengths;
+    int zero_rest; /* != 0: outputs' rows of no sequence get zeros */
+} dsp_gpu_linear_attention_shape;
+int dsp_gpu_linear_attention_workspace(const dsp_gpu_linear_attention_shape *shape, int backward, size_t *bytes);
+int dsp_gpu_linear_attention(const void *q, const void *k, const void *v, void *o,
+                             const dsp_gpu_linear_attention_shape *shape, const double *log_decay, double scale,
+                             const float *state_in, float *state_out, void *workspace, size_t workspace_bytes, void *stream);
+int dsp_gpu_linear_attention_backward(const void *q, const void *k, const void *v, const void *dout, void *dq, void *dk,
+                                      void *dv, const dsp_gpu_linear_attention_shape *shape, const double *log_decay,
+                                      double scale, const float *state_in, const float *dstate_out, float *dstate_in,
+                                      void *workspace, size_t workspace_bytes, void *stream);
+int dsp_gpu_linear_attention_step(const void *q, const void *k, const void *v, void *o,
+                                  const dsp_gpu_linear_attention_shape *shape, const double *log_decay, double scale,
+                                  float *state, const long long *slots, size_t n_slots, void *stream);
 
 /*
  * Local steps of the multi-GPU six-step FFT: one dsp::fft0 (fft.h:31-55) of N = N1*N2 points spread
