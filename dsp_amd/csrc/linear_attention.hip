@@ -13,8 +13,8 @@ namespace {
 
 // ---- segments -> states ------------------------------------------------------------------------------------------------
 
-// seg[s] holds what segment s leaves behind from a zero state; afterwards it holds the state segment s starts from, and
-// s_out the state after the last one.  One thread an element of the state; the loads do not depend on the recurrence.
+// seg[s] holds what segment s leaves behind from a zero state; afterwards it holds the state that segment s + 1 starts from.
+// One thread an element of the state; the loads do not depend on the recurrence.
 __global__ void __launch_bounds__(256) join_segments_kernel(const Args a) {
     const Role &role = a.role[blockIdx.y];
     const int count = role.d1 * role.d2, blocks = (count + 255) / 256;
@@ -22,26 +22,23 @@ __global__ void __launch_bounds__(256) join_segments_kernel(const Args a) {
     if (bh >= a.batch * a.heads || e >= count) return;
     long long start, len;
     sequence_rows(a, bh / a.heads, start, len);
-    const float log2w = a.log2_decay[bh % a.heads];
+    const int full = static_cast<int>((len - 1) / a.seg_len);  // segments with another one behind them (len = 0: none)
+    if (len == 0 || full == 0) return;
     float run = 0.0f;
     if (role.s_in) run = role.s_in[static_cast<size_t>(bh) * count + (e / role.d2) * role.s_in_d + (e % role.d2) * role.s_in_n];
-    float *seg = role.seg + static_cast<size_t>(bh) * a.segments * count + e;
-    const Decay whole = decay_over(log2w, a.seg_len);
-    for (int s0 = 0; s0 < a.segments; s0 += 8) {
+    float *seg = role.seg + static_cast<size_t>(bh) * (a.segments - 1) * count + e;
+    const Decay w = decay_over(a.log2_decay[bh % a.heads], a.seg_len);
+    for (int s0 = 0; s0 < full; s0 += 8) {
         float local[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)  // the last segment's own state is computed only where someone asks for it
-            local[i] = s0 + i < a.segments - (role.s_out ? 0 : 1) && (s0 + i) * a.seg_len < len ? seg[static_cast<size_t>(s0 + i) * count] : 0.0f;
+        for (int i = 0; i < 8; ++i) local[i] = s0 + i < full ? seg[static_cast<size_t>(s0 + i) * count] : 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const long long left = len - (s0 + i) * a.seg_len;
-            if (s0 + i >= a.segments || left <= 0) break;
-            seg[static_cast<size_t>(s0 + i) * count] = run;
-            const Decay w = left >= a.seg_len ? whole : decay_over(log2w, left);
+            if (s0 + i >= full) break;
             run = fmaf(run, w.hi, fmaf(run, w.lo, local[i]));
+            seg[static_cast<size_t>(s0 + i) * count] = run;
         }
     }
-    if (role.s_out) role.s_out[static_cast<size_t>(bh) * count + e] = run;
 }
 
 // ---- gradients of shared heads -----------------------------------------------------------------------------------------
@@ -287,49 +284,61 @@ struct Plan {
     long long seg_len;
 };
 
-constexpr size_t kFill = 512;  // workgroups that fill the chip: two on each of 256 CUs
+constexpr long long kSlots = 512;     // workgroups the chip runs at once: two on each of 256 CUs
+constexpr long long kLeast = 256;     // tokens of a segment at least: a state is written and read for each
 
 // How the work of `roles` runs over batch * heads sequences is spread.  A workgroup that owns 128 columns reads q and k half
-// as often as two that own 64, so columns are split only to fill the chip; then the time axis is cut into segments, which
-// costs a second pass over k and v, so the segments stay as few and as long as the chip allows.
+// as often as two that own 64.  Where the runs do not fill the chip the time axis is cut into segments, which costs a
+// second pass over k and v (about kAgain of the first): dense batches take the number of segments with the least
+// ceil(workgroups / slots) * tokens of a segment; of ragged ones only the sum of the lengths is known, and the segments
+// are such that it makes about three rounds of half-filled slots.
 Plan make_plan(const Shape &p, int d1, const int *d2, int roles) {
     Plan pl{};
     pl.d1p = d1 <= 64 ? 64 : d1 <= 128 ? 128 : 256;
-    const size_t runs = p.batch * static_cast<size_t>(p.heads);
-    auto groups = [&](int nt) {
-        size_t t = 0;
-        for (int r = 0; r < roles; ++r) t += (d2[r] + 64 * nt - 1) / (64 * nt);
-        return runs * t;
-    };
     bool wide = false;
     for (int r = 0; r < roles; ++r) wide = wide || d2[r] > 64;
     pl.nt = pl.d1p < 256 && wide ? 2 : 1;
-    const size_t w = groups(pl.nt);
-    const long long n = static_cast<long long>(p.offsets ? std::min(p.n, p.rows) : p.n), chunk = 64;
-    pl.segments = 1;
-    pl.seg_len = (n + chunk - 1) / chunk * chunk;
-    if (w < kFill / 2 && n >= 8 * chunk) {
-        const long long want = std::min<long long>(static_cast<long long>((kFill + w - 1) / w), n / (4 * chunk));
-        pl.seg_len = ((n + want - 1) / want + chunk - 1) / chunk * chunk;
-        pl.segments = static_cast<int>((n + pl.seg_len - 1) / pl.seg_len);
+    long long groups = 0;
+    for (int r = 0; r < roles; ++r) groups += (d2[r] + 64 * pl.nt - 1) / (64 * pl.nt);
+    groups *= p.heads;
+    const long long batch = static_cast<long long>(p.batch), n = static_cast<long long>(p.offsets ? std::min(p.n, p.rows) : p.n);
+    auto up = [](long long x) { return (x + 63) / 64 * 64; };  // whole chunks
+    pl.seg_len = std::max<long long>(64, up(n));
+    if (n >= 2 * kLeast) {
+        constexpr double kAgain = 0.4;
+        if (p.offsets) {
+            pl.seg_len = std::min(pl.seg_len, std::max(kLeast, up(static_cast<long long>(p.rows) * groups / (kSlots * 3 / 2))));
+        } else {
+            double best = 0.0;
+            for (long long s = 1; s <= 64 && s <= n / kLeast; ++s) {
+                const long long len = up((n + s - 1) / s), rounds = (batch * groups * ((n + len - 1) / len) + kSlots - 1) / kSlots;
+                const double cost = static_cast<double>(rounds * (len + 64)) * (s > 1 ? 1.0 + kAgain : 1.0);
+                if (s == 1 || cost < 0.9 * best) {
+                    best = cost;
+                    pl.seg_len = std::max<long long>(64, len);
+                }
+            }
+        }
     }
+    pl.segments = static_cast<int>(std::max<long long>(1, (n + pl.seg_len - 1) / pl.seg_len));
     return pl;
 }
 
 size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
 size_t segment_bytes(const Shape &p, const Plan &pl) {
-    return pl.segments > 1 ? align256(sizeof(float) * p.batch * p.heads * pl.segments * p.dim_k * p.dim_v) : 0;
+    return pl.segments > 1 ? align256(sizeof(float) * p.batch * p.heads * (pl.segments - 1) * p.dim_k * p.dim_v) : 0;
 }
 size_t total_rows(const Shape &p) { return p.offsets ? p.rows : p.batch * p.n; }
 size_t part_bytes(const Shape &p, int heads_x, int dim) {
     return heads_x < p.heads ? align256(sizeof(float) * total_rows(p) * p.heads * dim) : 0;
 }
 
-int launch_kernel(const Args &a, const Plan &pl, int type, unsigned blocks, bool state_only, hipStream_t s) {
-    if (type == DSP_GPU_BF16) return launch_bf16(a, pl.d1p, pl.nt, blocks, state_only, s);
-    if (type == DSP_GPU_F16) return launch_f16(a, pl.d1p, pl.nt, blocks, state_only, s);
-    return launch_f32(a, pl.d1p, pl.nt, blocks, state_only, s);
+int launch_kernel(const Args &a, const Variant &v, int type, size_t blocks, hipStream_t s) {
+    const unsigned n = static_cast<unsigned>(blocks);
+    if (type == DSP_GPU_BF16) return launch_bf16(a, v, n, s);
+    if (type == DSP_GPU_F16) return launch_f16(a, v, n, s);
+    return launch_f32(a, v, n, s);
 }
 
 // roles: a.role[0 .. a.roles) with everything but tiles and seg filled in; seg_ws: a.roles * segment_bytes
@@ -343,37 +352,35 @@ int run(const Shape &p, Args &a, const Plan &pl, char *seg_ws, hipStream_t s) {
     a.segments = pl.segments;
     a.seg_len = pl.seg_len;
     size_t tiles = 0, most = 0;
-    bool ends = false;
+    Variant v{pl.d1p, pl.nt, true, false};
     for (int r = 0; r < a.roles; ++r) {
         Role &x = a.role[r];
         x.tiles = (x.d2 + 64 * pl.nt - 1) / (64 * pl.nt);
         x.seg = pl.segments > 1 ? reinterpret_cast<float *>(seg_ws + r * segment_bytes(p, pl)) : nullptr;
         tiles += x.tiles;
         most = std::max<size_t>(most, (static_cast<size_t>(x.d1) * x.d2 + 255) / 256);
-        ends = ends || x.s_out;
+        v.vec = v.vec && x.vec;
     }
     const size_t runs = p.batch * p.heads, blocks = runs * tiles * pl.segments;
     if (blocks > 0x7fffffffu || runs * most > 0x7fffffffu) return fail(DSP_GPU_EINVAL, "linear attention: %zu workgroups", blocks);
     if (pl.segments > 1) {
-        if (int rc = launch_kernel(a, pl, p.sample_type, static_cast<unsigned>(runs * tiles * (pl.segments - (ends ? 0 : 1))), true, s)) return rc;
+        v.state_only = true;
+        if (int rc = launch_kernel(a, v, p.sample_type, runs * tiles * (pl.segments - 1), s)) return rc;
         join_segments_kernel<<<dim3(static_cast<unsigned>(runs * most), a.roles), 256, 0, s>>>(a);
         if (int rc = check_launch("join_segments_kernel")) return rc;
+        v.state_only = false;
     }
-    return launch_kernel(a, pl, p.sample_type, static_cast<unsigned>(blocks), false, s);
+    return launch_kernel(a, v, p.sample_type, blocks, s);
 }
 
 void set_strides(long long *to, const long long *from) {
     for (int i = 0; i < 3; ++i) to[i] = from[i];
 }
 
-// 16-byte accesses of a tensor: whole packs in a row, and every row aligned
-bool packs(const void *p, const long long *stride, int dim, int type) {
-    const long long ve = type == DSP_GPU_BF16 ? 8 : 4;
-    const size_t align = ve * sample_bytes(type);
-    return reinterpret_cast<uintptr_t>(p) % align == 0 && dim % ve == 0 && stride[0] % ve == 0 && stride[1] % ve == 0 && stride[2] % ve == 0;
-}
-bool quads(const void *p, const long long *stride, int dim, size_t size) {
-    return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && dim % 4 == 0 && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[2] % 4 == 0;
+// Rows of whole packs of `ve` elements, aligned, and a chunk's 64 rows within 2^29 bytes of one another
+bool packs(const void *p, const long long *stride, int dim, long long ve, size_t size) {
+    return reinterpret_cast<uintptr_t>(p) % (ve * size) == 0 && dim % ve == 0 && stride[0] % ve == 0 && stride[1] % ve == 0 &&
+           stride[2] % ve == 0 && stride[1] < (1ll << 21);
 }
 
 struct Tensor {
@@ -388,8 +395,10 @@ void fill_role(Role &r, const Shape &p, const Tensor &q, const Tensor &k, const 
     r.q_group = p.heads / q.heads, r.k_group = p.heads / k.heads, r.v_group = p.heads / v.heads;
     r.d1 = q.dim, r.d2 = v.dim;
     r.o_partial = partial;
-    r.vec = packs(q.p, q.stride, q.dim, p.sample_type) | packs(k.p, k.stride, k.dim, p.sample_type) << 1 |
-            packs(v.p, v.stride, v.dim, p.sample_type) << 2 | quads(o, o_stride, v.dim, partial ? 4 : sample_bytes(p.sample_type)) << 3;
+    const size_t size = sample_bytes(p.sample_type);
+    const long long ve = p.sample_type == DSP_GPU_BF16 ? 8 : 4;
+    r.vec = packs(q.p, q.stride, q.dim, ve, size) && packs(k.p, k.stride, k.dim, ve, size) && packs(v.p, v.stride, v.dim, ve, size) &&
+            packs(o, o_stride, v.dim, 4, partial ? 4 : size);
 }
 
 struct BackwardPlan {

@@ -4,8 +4,8 @@
 namespace dspgpu {
 namespace la {
 
-int launch_bf16(const Args &a, int d1p, int nt, unsigned blocks, bool state_only, hipStream_t s) {
-    return launch_any<__bf16, __bf16>(a, d1p, nt, blocks, state_only, s);
+int launch_bf16(const Args &a, const Variant &v, unsigned blocks, hipStream_t s) {
+    return launch_any<__bf16, __bf16>(a, v, blocks, s);
 }
 
 }  // namespace la

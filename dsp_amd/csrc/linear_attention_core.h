@@ -3,8 +3,10 @@
 // One head of one sequence, w = its decay, S the [d1][d2] state, tokens taken in chunks of C (in reverse time for the
 // gradients of k and v):
 //     P[i][j] = w^{i-j} (q_i . k_j) scale      for j <= i, else 0
-//     O[i]    = w^{i+1-late} read * q_i S + sum_j P[i][j] v_j
-//     S      <- w^C S + sum_j w^{C-1-j+late} write * k_j v_j^T
+//     O[i]    = w^{i+1} read * q_i S + sum_j P[i][j] v_j
+//     S      <- w^C S + sum_j w^{C-1-j} write * k_j v_j^T
+// In reverse time the chunks come last to first, the tokens of one stay in their places, and every weight is mirrored:
+//     P[i][j] = w^{j-i} ... for j >= i,   O[i] = w^{C-1-i} read ...,   S <- w^C S + sum_j w^{j+1} write ...
 // A workgroup of four waves keeps the d1 x (64 NT) part of S in fp32 accumulators for its whole run over the tokens, so
 // that the state never travels: q, k, v are read and o is written once.  Wave w owns 16 NT columns of S and of O.
 //
@@ -45,12 +47,12 @@ struct Role {
     int d1, d2, tiles;             // tiles of 64 NT columns
     int late;                      // 1: reverse time
     int o_partial;
-    int vec;                       // bit 0..3: q, k, v, o take 16-byte (o: 4-element) accesses
+    int vec;                       // rows of q, k, v are whole aligned packs, rows of o whole aligned quads
     float read, write, pscale;
     const float *s_in;             // [sequence][head] blocks of d1 * d2, element (d, n) at d * s_in_d + n * s_in_n; or null
     int s_in_d, s_in_n;
     float *s_out;                  // [sequence][head][d1][d2] or null
-    float *seg;                    // [sequence * heads + head][segments][d1][d2]: states of the segments (null: one segment)
+    float *seg;                    // [sequence * heads + head][segments - 1][d1][d2]: states between the segments
 };
 
 struct Args {
@@ -114,6 +116,19 @@ __device__ __forceinline__ void mma(f32x4 &acc, f32x8 a, f32x8 b) {
     for (int e = 0; e < 8; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], acc, 0, 0, 0);
 }
 
+// Sixteen wait states between matrix products and whatever reads their results after them (eleven are needed).  hipcc 7.2
+// leaves them out where the reader opens a block behind two uniform branches: halves of accumulators were stored stale.
+__device__ __forceinline__ void settle(f32x4 &a) { asm volatile("s_nop 7\n\ts_nop 7" : "+v"(a)); }
+__device__ __forceinline__ void settle(f32x4 &a, f32x4 &b) { asm volatile("s_nop 7\n\ts_nop 7" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ void settle(f32x4 &a, f32x4 &b, f32x4 &c, f32x4 &d) { asm volatile("s_nop 7\n\ts_nop 7" : "+v"(a), "+v"(b), "+v"(c), "+v"(d)); }
+template <int N>
+__device__ __forceinline__ void settle(f32x4 (&x)[N]) {
+    if constexpr (N >= 8) asm volatile("s_nop 7\n\ts_nop 7" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]));
+    if constexpr (N == 16) asm volatile("s_nop 7\n\ts_nop 7" : "+v"(x[8]), "+v"(x[9]), "+v"(x[10]), "+v"(x[11]), "+v"(x[12]), "+v"(x[13]), "+v"(x[14]), "+v"(x[15]));
+    if constexpr (N == 4) settle(x[0], x[1], x[2], x[3]);
+    if constexpr (N == 2) settle(x[0], x[1]);
+}
+
 // 8 contraction elements of one row: columns 4g .. 4g+3 and 16 + 4g .. of the 32 at p (p: the row's first of these 32)
 __device__ __forceinline__ bf16x8 row_frag(const __bf16 *p, int g) {
     const bf16x4 a = *reinterpret_cast<const bf16x4 *>(p + 4 * g), b = *reinterpret_cast<const bf16x4 *>(p + 16 + 4 * g);
@@ -164,19 +179,29 @@ struct Pack {
     T e[N];
 };
 
-// VE consecutive elements of a row, zeros from column `cols` on
+// Rows are reached through buffer descriptors that start at a chunk's first row: a lane whose row or column lies outside
+// gets an offset past the descriptor's end, reads zeros and writes nothing, and no load or store sits behind a branch.
+// (Offset and step are below 2^29 each for everything inside, so the end is out of reach for those.)
+constexpr int kRecords = 0x7fffffff;
+constexpr unsigned kOutside = 0xc0000000u;  // with or without a step
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(const void *p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, kRecords, 0x00027000);
+}
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 template <typename Ti, int VE>
-__device__ __forceinline__ Pack<Ti, VE> load_pack(const Ti *row, int col, int cols, bool vec) {
+__device__ __forceinline__ Pack<Ti, VE> load_pack(__amdgpu_buffer_rsrc_t r, unsigned offset, int step) {
+    if constexpr (sizeof(Ti) * VE == 16) return __builtin_bit_cast(Pack<Ti, VE>, __builtin_amdgcn_raw_buffer_load_b128(r, offset, step, 0));
+    else return __builtin_bit_cast(Pack<Ti, VE>, __builtin_amdgcn_raw_buffer_load_b64(r, offset, step, 0));
+}
+// the same element by element, for rows that are not whole aligned packs: the first `left` of VE, zeros behind them
+template <typename Ti, int VE>
+__device__ __forceinline__ Pack<Ti, VE> load_elements(const Ti *p, int left) {
     Pack<Ti, VE> r;
-    typedef int raw __attribute__((ext_vector_type(VE * sizeof(Ti) / 4)));
-    if (vec) {  // cols is a multiple of VE and the row aligned
-        raw v = {};
-        if (col < cols) v = *reinterpret_cast<const raw *>(row + col);
-        __builtin_memcpy(&r, &v, sizeof r);
-    } else {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) r.e[e] = col + e < cols ? row[col + e] : static_cast<Ti>(0.0f);
-    }
+    for (int e = 0; e < VE; ++e) r.e[e] = e < left ? p[e] : static_cast<Ti>(0.0f);
     return r;
 }
 
@@ -187,20 +212,27 @@ __device__ __forceinline__ void to_lds(float *p, const Pack<_Float16, 4> &v) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store4(T *p, const f32x4 &v, int left, bool vec) {
-    if (vec) {
-        if (left >= 4) {
-            typedef T t4 __attribute__((ext_vector_type(4)));
-            t4 o;
+__device__ __forceinline__ void to_lds4(T *p, const f32x4 &v) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 o;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(v[r]);
-            *reinterpret_cast<t4 *>(p) = o;
-        }
-    } else {
+    for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(v[r]);
+    *reinterpret_cast<t4 *>(p) = o;
+}
+template <typename T>
+__device__ __forceinline__ void store_quad(__amdgpu_buffer_rsrc_t r, unsigned offset, int step, const f32x4 &v) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 o;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (r < left) p[r] = static_cast<T>(v[r]);
-    }
+    for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(v[e]);
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, o), r, offset, step, 0);
+    else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(i32x2, o), r, offset, step, 0);
+}
+template <typename T>
+__device__ __forceinline__ void store_elements(T *p, const f32x4 &v, int left) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (r < left) p[r] = static_cast<T>(v[r]);
 }
 
 // ---- the kernel ------------------------------------------------------------------------------------------------------
@@ -213,7 +245,7 @@ struct Lds {
     Tc k[C * kD];
     Tc v[C * kN];
     Tc p[C * kP];
-    float pw[C + 4];
+    float pw[2 * C + 4];  // w^|x| at C + x
 };
 template <typename Tc, int D1P, int NT, int C>
 struct LdsState {  // no queries
@@ -221,18 +253,20 @@ struct LdsState {  // no queries
     static constexpr int kD = D1P + kPad, kN = 64 * NT + kPad, kP = 0;
     Tc k[C * kD];
     Tc v[C * kN];
-    float pw[C + 4];
+    float pw[2 * C + 4];
 };
 
-// STATE_ONLY: the state a segment leaves behind when it starts from zero -> seg[segment]
-template <typename Ti, typename Tc, int D1P, int NT, int C, bool STATE_ONLY>
+// STATE_ONLY: the state a segment leaves behind when it starts from zero -> seg[segment], for all but a sequence's last.
+// VEC: rows of q, k, v are whole aligned packs, rows of o whole aligned quads, and a chunk of any of them spans < 2^29 bytes.
+template <typename Ti, typename Tc, int D1P, int NT, int C, bool STATE_ONLY, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Args a) {
     using F = typename Cfg<Tc>::frag;
     using L = typename std::conditional<STATE_ONLY, LdsState<Tc, D1P, NT, C>, Lds<Tc, D1P, NT, C>>::type;
     constexpr int VE = Cfg<Tc>::kVe;
     constexpr int KB = D1P / 32, DT = D1P / 16, IT = C / 16, JB = C / 32, NB = 64 * NT;
-    constexpr int QV = C * D1P / VE / kThreads, VV = C * NB / VE / kThreads;  // packs a thread moves
-    static_assert(QV * VE * kThreads == C * D1P && VV * VE * kThreads == C * NB, "whole packs");
+    constexpr int QV = C * D1P / VE / kThreads, VV = C * NB / VE / kThreads;      // packs a thread moves
+    constexpr int QROWS = kThreads * VE / D1P, VROWS = kThreads * VE / NB;        // rows between them
+    static_assert(QV * QROWS == C && VV * VROWS == C, "whole packs");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     L &lds = *reinterpret_cast<L *>(smem);
 
@@ -254,36 +288,39 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
     long long start, len;
     sequence_rows(a, b, start, len);
     const long long u0 = segment * a.seg_len, u1 = min(len, u0 + a.seg_len);  // in the order of traversal
-    const bool split = role.seg != nullptr;
-    if (u0 >= u1 && (split || !role.s_out)) return;  // an empty sequence still hands its state on
+    if (STATE_ONLY && u1 >= len) return;
+    if (u0 >= u1 && (segment > 0 || !role.s_out)) return;  // an empty sequence still hands its state on
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
-    const int d1 = role.d1, d2 = role.d2;
-    const float log2w = a.log2_decay[head];
+    const int d1 = role.d1, d2 = role.d2, late = role.late;
+    const float log2w = a.log2_decay[head], read = role.read, write = role.write, pscale = role.pscale;
     const size_t bh = static_cast<size_t>(b) * a.heads + head;
     const long long base = a.offsets ? 0 : b;  // packed rows have no sequence stride
-    const Ti *q = static_cast<const Ti *>(role.q) + base * role.qs[0] + start * role.qs[1] + (head / role.q_group) * role.qs[2];
-    const Ti *k = static_cast<const Ti *>(role.k) + base * role.ks[0] + start * role.ks[1] + (head / role.k_group) * role.ks[2];
-    const Ti *v = static_cast<const Ti *>(role.v) + base * role.vs[0] + start * role.vs[1] + (head / role.v_group) * role.vs[2] + n0;
-    const bool qvec = role.vec & 1, kvec = role.vec & 2, vvec = role.vec & 4, ovec = role.vec & 8;
+    const long long qt = role.qs[1], kt = role.ks[1], vt = role.vs[1], ot = role.os[1];
+    const Ti *q = static_cast<const Ti *>(role.q) + base * role.qs[0] + start * qt + (head / role.q_group) * role.qs[2];
+    const Ti *k = static_cast<const Ti *>(role.k) + base * role.ks[0] + start * kt + (head / role.k_group) * role.ks[2];
+    const Ti *v = static_cast<const Ti *>(role.v) + base * role.vs[0] + start * vt + (head / role.v_group) * role.vs[2] + n0;
+    const bool partial = role.o_partial;
+    const int osize = partial ? 4 : static_cast<int>(sizeof(Ti));
+    char *o = static_cast<char *>(role.o) + (base * role.os[0] + start * ot + head * role.os[2] + n0) * osize;
 
-    if (tid <= C) lds.pw[tid] = power(log2w, static_cast<float>(tid));
+    for (int x = tid; x <= 2 * C; x += kThreads) lds.pw[x] = power(log2w, static_cast<float>(x < C ? C - x : x - C));
 
     // the state: lane holds rows 16 dt + 4g + r, column n0 + 16 (NT wave + nt) + m
-    f32x4 S[DT][NT];
+    f32x4 S[DT * NT];
     {
         const float *s_in = nullptr;
-        size_t sd = 0, sn = 1;
+        int sd = d2, sn = 1;
         if constexpr (!STATE_ONLY) {
-            if (split) {
-                s_in = role.seg + (bh * a.segments + segment) * d1 * d2;
-                sd = d2;
+            if (segment > 0) {
+                s_in = role.seg + (bh * (a.segments - 1) + segment - 1) * d1 * d2;
             } else if (role.s_in) {
                 s_in = role.s_in + bh * d1 * d2;
                 sd = role.s_in_d;
                 sn = role.s_in_n;
             }
         }
+        const auto from = descriptor(s_in);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -292,57 +329,78 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int d = 16 * dt + 4 * g + r;
-                    S[dt][nt][r] = s_in && d < d1 && n < d2 ? s_in[d * sd + n * sn] : 0.0f;
+                    const unsigned at = s_in && d < d1 && n < d2 ? (d * sd + n * sn) * 4u : kOutside;
+                    S[dt * NT + nt][r] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0));
                 }
             }
     }
 
+    const int qrow = tid * VE / D1P, qcol = tid * VE % D1P, vrow = tid * VE / NB, vcol = tid * VE % NB;
+    constexpr int es = sizeof(Ti);
+    unsigned qoff = 0, koff = 0, voff = 0;
+    if constexpr (VEC) {
+        qoff = qcol < d1 ? (qrow * static_cast<int>(qt) + qcol) * es : kOutside;
+        koff = qcol < d1 ? (qrow * static_cast<int>(kt) + qcol) * es : kOutside;
+        voff = n0 + vcol < d2 ? (vrow * static_cast<int>(vt) + vcol) * es : kOutside;
+    }
+
+    // the `size` tokens from u on in the order of traversal: the lowest of them
+    auto lowest = [&](long long u, int size) { return late ? len - u - size : u; };
     Pack<Ti, VE> rq[STATE_ONLY ? 1 : QV], rk[QV], rv[VV];
-    // rows u .. u + C of the traversal into registers, zeros behind the last one
-    auto fetch = [&](long long u) {
+    // their rows into registers, zeros behind the last one
+    auto fetch = [&](long long u, int size) {
+        const long long low = lowest(u, size);
+        if constexpr (VEC) {
+            const auto dq = descriptor(q + low * qt), dk = descriptor(k + low * kt), dv = descriptor(v + low * vt);
 #pragma unroll
-        for (int x = 0; x < QV; ++x) {
-            const int at = (x * kThreads + tid) * VE, row = at / D1P, col = at % D1P;
-            const long long uu = u + row, tt = role.late ? len - 1 - uu : uu;
-            const bool in = uu < u1;
-            rk[x] = load_pack<Ti, VE>(k + (in ? tt : 0) * role.ks[1], col, in ? d1 : 0, kvec);
-            if constexpr (!STATE_ONLY) rq[x] = load_pack<Ti, VE>(q + (in ? tt : 0) * role.qs[1], col, in ? d1 : 0, qvec);
-        }
+            for (int x = 0; x < QV; ++x) {
+                const bool in = qrow < size - x * QROWS;
+                rk[x] = load_pack<Ti, VE>(dk, in ? koff : kOutside, x * QROWS * es * static_cast<int>(kt));
+                if constexpr (!STATE_ONLY) rq[x] = load_pack<Ti, VE>(dq, in ? qoff : kOutside, x * QROWS * es * static_cast<int>(qt));
+            }
 #pragma unroll
-        for (int x = 0; x < VV; ++x) {
-            const int at = (x * kThreads + tid) * VE, row = at / NB, col = at % NB;
-            const long long uu = u + row, tt = role.late ? len - 1 - uu : uu;
-            const bool in = uu < u1;
-            rv[x] = load_pack<Ti, VE>(v + (in ? tt : 0) * role.vs[1], col, in ? d2 - n0 : 0, vvec);
+            for (int x = 0; x < VV; ++x)
+                rv[x] = load_pack<Ti, VE>(dv, vrow < size - x * VROWS ? voff : kOutside, x * VROWS * es * static_cast<int>(vt));
+        } else {
+#pragma unroll
+            for (int x = 0; x < QV; ++x) {
+                const int row = qrow + x * QROWS;
+                rk[x] = load_elements<Ti, VE>(k + (low + row) * kt + qcol, row < size ? d1 - qcol : 0);
+                if constexpr (!STATE_ONLY) rq[x] = load_elements<Ti, VE>(q + (low + row) * qt + qcol, row < size ? d1 - qcol : 0);
+            }
+#pragma unroll
+            for (int x = 0; x < VV; ++x) {
+                const int row = vrow + x * VROWS;
+                rv[x] = load_elements<Ti, VE>(v + (low + row) * vt + vcol, row < size ? d2 - n0 - vcol : 0);
+            }
         }
     };
     auto commit = [&]() {
 #pragma unroll
         for (int x = 0; x < QV; ++x) {
-            const int at = (x * kThreads + tid) * VE, row = at / D1P, col = at % D1P;
-            to_lds(lds.k + row * L::kD + col, rk[x]);
-            if constexpr (!STATE_ONLY) to_lds(lds.q + row * L::kD + col, rq[x]);
+            to_lds(lds.k + (qrow + x * QROWS) * L::kD + qcol, rk[x]);
+            if constexpr (!STATE_ONLY) to_lds(lds.q + (qrow + x * QROWS) * L::kD + qcol, rq[x]);
         }
 #pragma unroll
-        for (int x = 0; x < VV; ++x) {
-            const int at = (x * kThreads + tid) * VE, row = at / NB, col = at % NB;
-            to_lds(lds.v + row * L::kN + col, rv[x]);
-        }
+        for (int x = 0; x < VV; ++x) to_lds(lds.v + (vrow + x * VROWS) * L::kN + vcol, rv[x]);
     };
+    auto size_at = [&](long long u) { return static_cast<int>(min(static_cast<long long>(C), u1 - u)); };
 
     const Decay whole = decay_over(log2w, C);
     if (u0 < u1) {
-        fetch(u0);
+        fetch(u0, size_at(u0));
         commit();
     }
     __syncthreads();
 
     for (long long u = u0; u < u1; u += C) {
-        const int size = static_cast<int>(min(static_cast<long long>(C), u1 - u));
+        const int size = size_at(u);
         const bool more = u + C < u1;
-        if (more) fetch(u + C);
+        if (more) fetch(u + C, size_at(u + C));
 
-        f32x4 O[STATE_ONLY ? 1 : IT][NT];
+        const float *const pw_mirrored = lds.pw + C - (size - 1), *const pw_plain = lds.pw + C + 1;
+        const float *const pw_read = late ? pw_mirrored : pw_plain, *const pw_write = late ? pw_plain : pw_mirrored;
+        f32x4 O[STATE_ONLY ? 2 : IT * NT];
         if constexpr (!STATE_ONLY) {
             // P^T = K Q^T: wave w takes the keys of tile w % IT for every (4 / IT)-th tile of queries
             const int jt = wave % IT;
@@ -351,34 +409,38 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
             for (int kb = 0; kb < KB; ++kb) {
                 kf[kb] = row_frag(lds.k + (16 * jt + m) * L::kD + 32 * kb, g);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) sf[kb][nt] = operand(S[2 * kb][nt], S[2 * kb + 1][nt], Tc());
+                for (int nt = 0; nt < NT; ++nt) sf[kb][nt] = operand(S[2 * kb * NT + nt], S[(2 * kb + 1) * NT + nt], Tc());
             }
 #pragma unroll
             for (int it = 0; it < IT; ++it) {
-                F qf[KB];
+                const bool mine = it % (4 / IT) == wave / IT;
+                f32x4 p = {};
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) qf[kb] = row_frag(lds.q + (16 * it + m) * L::kD + 32 * kb, g);
-                const float rd = role.read * lds.pw[16 * it + m + 1 - role.late];
+                for (int nt = 0; nt < NT; ++nt) O[it * NT + nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    f32x4 acc = {};
+                for (int kb = 0; kb < KB; ++kb) {
+                    const F qf = row_frag(lds.q + (16 * it + m) * L::kD + 32 * kb, g);
 #pragma unroll
-                    for (int kb = 0; kb < KB; ++kb) mma(acc, sf[kb][nt], qf[kb]);
-                    O[it][nt] = acc * rd;
+                    for (int nt = 0; nt < NT; ++nt) mma(O[it * NT + nt], sf[kb][nt], qf);
+                    if (mine && (late ? jt >= it : jt <= it)) mma(p, kf[kb], qf);
                 }
-                if (it % (4 / IT) == wave / IT && jt / 2 <= it / 2) {
-                    f32x4 p = {};
-                    if (jt <= it) {
-#pragma unroll
-                        for (int kb = 0; kb < KB; ++kb) mma(p, kf[kb], qf[kb]);
-                    }
+                if (mine && (late ? jt / 2 >= it / 2 : jt / 2 <= it / 2)) {
+                    settle(p);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int gap = 16 * (it - jt) + m - 4 * g - r;
-                        p[r] = gap >= 0 ? p[r] * (role.pscale * lds.pw[gap < 0 ? 0 : gap]) : 0.0f;
+                        const float w = pscale * lds.pw[C + gap];
+                        p[r] = (late ? -gap : gap) >= 0 ? p[r] * w : 0.0f;
                     }
-                    store4(lds.p + (16 * it + m) * L::kP + 16 * jt + 4 * g, p, 4, true);
+                    to_lds4(lds.p + (16 * it + m) * L::kP + 16 * jt + 4 * g, p);
                 }
+            }
+            settle(O);
+#pragma unroll
+            for (int it = 0; it < IT; ++it) {
+                const float rd = read * pw_read[16 * it + m];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) O[it * NT + nt] *= rd;
             }
             __syncthreads();
         }
@@ -390,42 +452,50 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
             for (int nt = 0; nt < NT; ++nt) vf[jb][nt] = col_frag<L::kN>(lds.v + 32 * jb * L::kN + 16 * (NT * wave + nt), g, m);
 
         if constexpr (!STATE_ONLY) {
+            char *const op = o + lowest(u, size) * ot * osize;
+            const auto dout = descriptor(op);
 #pragma unroll
             for (int it = 0; it < IT; ++it) {
 #pragma unroll
-                for (int jb = 0; jb <= it / 2; ++jb) {
+                for (int jb = 0; jb < JB; ++jb) {
+                    if (late ? jb < it / 2 : jb > it / 2) continue;
                     const F pf = row_frag(lds.p + (16 * it + m) * L::kP + 32 * jb, g);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma(O[it][nt], vf[jb][nt], pf);
+                    for (int nt = 0; nt < NT; ++nt) mma(O[it * NT + nt], vf[jb][nt], pf);
                 }
-                if (16 * it + m < size) {
-                    const long long uu = u + 16 * it + m, tt = start + (role.late ? len - 1 - uu : uu);
+            }
+            settle(O);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const int n = n0 + 16 * (NT * wave + nt) + 4 * g;
-                        const long long at = base * role.os[0] + tt * role.os[1] + head * role.os[2] + n;
-                        if (role.o_partial) store4(static_cast<float *>(role.o) + at, O[it][nt], d2 - n, ovec);
-                        else store4(static_cast<Ti *>(role.o) + at, O[it][nt], d2 - n, ovec);
+            for (int it = 0; it < IT; ++it) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const int n = 16 * (NT * wave + nt) + 4 * g;
+                    if constexpr (VEC) {
+                        const unsigned at = m < size - 16 * it && n0 + n < d2 ? (m * static_cast<int>(ot) + n) * osize : kOutside;
+                        const int step = 16 * it * static_cast<int>(ot) * osize;
+                        if (partial) store_quad<float>(dout, at, step, O[it * NT + nt]);
+                        else store_quad<Ti>(dout, at, step, O[it * NT + nt]);
+                    } else if (16 * it + m < size) {
+                        char *const to = op + ((16 * it + m) * ot + n) * osize;
+                        if (partial) store_elements(reinterpret_cast<float *>(to), O[it * NT + nt], d2 - n0 - n);
+                        else store_elements(reinterpret_cast<Ti *>(to), O[it * NT + nt], d2 - n0 - n);
                     }
                 }
             }
         }
 
-        // S <- w^size S + K^T diag(w^{size-1-j+late} write) V, the weighted V in three bf16 parts (fp32: in one)
+        // S <- w^size S + K^T (weighted V), the weighted V in three bf16 parts (fp32: in one); rows behind the last are zeros
         const Decay wc = size == C ? whole : decay_over(log2w, size);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) S[dt][nt] = S[dt][nt] * wc.hi + S[dt][nt] * wc.lo;
+            for (int nt = 0; nt < NT; ++nt) S[dt * NT + nt] = S[dt * NT + nt] * wc.hi + S[dt * NT + nt] * wc.lo;
 #pragma unroll
         for (int jb = 0; jb < JB; ++jb) {
             float wj[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int j = 32 * jb + 16 * (e >> 2) + 4 * g + (e & 3);
-                wj[e] = j < size ? role.write * lds.pw[size - 1 - j + role.late] : 0.0f;
-            }
-            constexpr int PARTS = sizeof(Tc) == 2 ? 3 : 1;
+            for (int e = 0; e < 8; ++e) wj[e] = write * pw_write[32 * jb + 16 * (e >> 2) + 4 * g + (e & 3)];
+            constexpr int PARTS = sizeof(Tc) == 2 ? 3 : 1, GROUP = 4;
             F part[PARTS][NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -439,14 +509,19 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
                     }
                 }
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const F kt = col_frag<L::kD>(lds.k + 32 * jb * L::kD + 16 * dt, g, m);
+            for (int d0 = 0; d0 < DT; d0 += GROUP) {  // four tiles of rows at a time: products that do not wait for each other
+                F kc[GROUP];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int i = 0; i < GROUP; ++i) kc[i] = col_frag<L::kD>(lds.k + 32 * jb * L::kD + 16 * (d0 + i), g, m);
 #pragma unroll
-                    for (int s = PARTS - 1; s >= 0; --s) mma(S[dt][nt], kt, part[s][nt]);
+                for (int s = PARTS - 1; s >= 0; --s)
+#pragma unroll
+                    for (int i = 0; i < GROUP; ++i)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma(S[(d0 + i) * NT + nt], kc[i], part[s][nt]);
             }
         }
+        settle(S);
         __syncthreads();
         if (more) {
             commit();
@@ -455,9 +530,12 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
     }
 
     float *s_out = nullptr;
-    if constexpr (STATE_ONLY) s_out = role.seg + (bh * a.segments + segment) * d1 * d2;
-    else if (!split && role.s_out) s_out = role.s_out + bh * d1 * d2;
+    if constexpr (STATE_ONLY) s_out = role.seg + (bh * (a.segments - 1) + segment) * d1 * d2;
+    else if (role.s_out && u1 == len) s_out = role.s_out + bh * d1 * d2;
     if (s_out) {
+        int rows = d1, cols = d2;  // hidden from the compiler, which would keep 64 comparisons of the loads above for the stores
+        asm volatile("" : "+s"(rows), "+s"(cols));
+        const auto to = descriptor(s_out);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -466,43 +544,47 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int d = 16 * dt + 4 * g + r;
-                    if (d < d1 && n < d2) s_out[static_cast<size_t>(d) * d2 + n] = S[dt][nt][r];
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(S[dt * NT + nt][r]), to,
+                                                          d < rows && n < cols ? (d * cols + n) * 4u : kOutside, 0, 0);
                 }
             }
     }
 }
 
 // D1P and NT by the host's rule; C by the type: 64 tokens, 32 where an element is four bytes or a row 256 of them (LDS)
-template <typename Ti, typename Tc, int D1P, int NT>
-int launch_one(const Args &a, unsigned blocks, bool state_only, hipStream_t s) {
+template <typename Ti, typename Tc, int D1P, int NT, bool STATE_ONLY, bool VEC>
+int launch_kernel_as(const Args &a, unsigned blocks, hipStream_t s) {
     constexpr int C = sizeof(Tc) == 2 && D1P <= 128 ? 64 : 32;
-    if (state_only) {
-        using L = LdsState<Tc, D1P, NT, C>;
-        const auto fn = linear_attention_kernel<Ti, Tc, D1P, NT, C, true>;
-        if (sizeof(L) > 65536)
-            if (int rc = allow_full_lds(reinterpret_cast<const void *>(fn))) return rc;
-        fn<<<blocks, kThreads, sizeof(L), s>>>(a);
-    } else {
-        using L = Lds<Tc, D1P, NT, C>;
-        const auto fn = linear_attention_kernel<Ti, Tc, D1P, NT, C, false>;
-        if (sizeof(L) > 65536)
-            if (int rc = allow_full_lds(reinterpret_cast<const void *>(fn))) return rc;
-        fn<<<blocks, kThreads, sizeof(L), s>>>(a);
-    }
+    using L = typename std::conditional<STATE_ONLY, LdsState<Tc, D1P, NT, C>, Lds<Tc, D1P, NT, C>>::type;
+    const auto fn = linear_attention_kernel<Ti, Tc, D1P, NT, C, STATE_ONLY, VEC>;
+    if (sizeof(L) > 65536)
+        if (int rc = allow_full_lds(reinterpret_cast<const void *>(fn))) return rc;
+    fn<<<blocks, kThreads, sizeof(L), s>>>(a);
     return check_launch("linear_attention_kernel");
 }
 
+struct Variant {
+    int d1p, nt;
+    bool vec, state_only;
+};
+
+template <typename Ti, typename Tc, int D1P, int NT>
+int launch_one(const Args &a, const Variant &v, unsigned blocks, hipStream_t s) {
+    if (v.state_only) return v.vec ? launch_kernel_as<Ti, Tc, D1P, NT, true, true>(a, blocks, s) : launch_kernel_as<Ti, Tc, D1P, NT, true, false>(a, blocks, s);
+    return v.vec ? launch_kernel_as<Ti, Tc, D1P, NT, false, true>(a, blocks, s) : launch_kernel_as<Ti, Tc, D1P, NT, false, false>(a, blocks, s);
+}
+
 template <typename Ti, typename Tc>
-int launch_any(const Args &a, int d1p, int nt, unsigned blocks, bool state_only, hipStream_t s) {
-    if (d1p == 64) return nt == 1 ? launch_one<Ti, Tc, 64, 1>(a, blocks, state_only, s) : launch_one<Ti, Tc, 64, 2>(a, blocks, state_only, s);
-    if (d1p == 128) return nt == 1 ? launch_one<Ti, Tc, 128, 1>(a, blocks, state_only, s) : launch_one<Ti, Tc, 128, 2>(a, blocks, state_only, s);
-    return launch_one<Ti, Tc, 256, 1>(a, blocks, state_only, s);
+int launch_any(const Args &a, const Variant &v, unsigned blocks, hipStream_t s) {
+    if (v.d1p == 64) return v.nt == 1 ? launch_one<Ti, Tc, 64, 1>(a, v, blocks, s) : launch_one<Ti, Tc, 64, 2>(a, v, blocks, s);
+    if (v.d1p == 128) return v.nt == 1 ? launch_one<Ti, Tc, 128, 1>(a, v, blocks, s) : launch_one<Ti, Tc, 128, 2>(a, v, blocks, s);
+    return launch_one<Ti, Tc, 256, 1>(a, v, blocks, s);
 }
 
 // one translation unit each
-int launch_bf16(const Args &a, int d1p, int nt, unsigned blocks, bool state_only, hipStream_t s);
-int launch_f16(const Args &a, int d1p, int nt, unsigned blocks, bool state_only, hipStream_t s);
-int launch_f32(const Args &a, int d1p, int nt, unsigned blocks, bool state_only, hipStream_t s);
+int launch_bf16(const Args &a, const Variant &v, unsigned blocks, hipStream_t s);
+int launch_f16(const Args &a, const Variant &v, unsigned blocks, hipStream_t s);
+int launch_f32(const Args &a, const Variant &v, unsigned blocks, hipStream_t s);
 
 }  // namespace la
 }  // namespace dspgpu

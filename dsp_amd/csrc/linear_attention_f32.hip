@@ -4,8 +4,8 @@
 namespace dspgpu {
 namespace la {
 
-int launch_f32(const Args &a, int d1p, int nt, unsigned blocks, bool state_only, hipStream_t s) {
-    return launch_any<float, float>(a, d1p, nt, blocks, state_only, s);
+int launch_f32(const Args &a, const Variant &v, unsigned blocks, hipStream_t s) {
+    return launch_any<float, float>(a, v, blocks, s);
 }
 
 }  // namespace la
