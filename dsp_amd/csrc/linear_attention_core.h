@@ -102,12 +102,12 @@ struct Cfg;
 template <>
 struct Cfg<__bf16> {
     typedef bf16x8 frag;
-    static constexpr int kVe = 8, kPad = 8;
+    static constexpr int kVe = 8, kPad = 8, kPadT = 16;  // of rows read along / across: no two lanes of 32 share a bank
 };
 template <>
 struct Cfg<float> {
     typedef f32x8 frag;
-    static constexpr int kVe = 4, kPad = 4;
+    static constexpr int kVe = 4, kPad = 4, kPadT = 4;
 };
 
 __device__ __forceinline__ void mma(f32x4 &acc, bf16x8 a, bf16x8 b) { acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0); }
@@ -239,18 +239,19 @@ __device__ __forceinline__ void store_elements(T *p, const f32x4 &v, int left) {
 
 template <typename Tc, int D1P, int NT, int C>
 struct Lds {
-    static constexpr int kPad = Cfg<Tc>::kPad;
-    static constexpr int kD = D1P + kPad, kN = 64 * NT + kPad, kP = C + kPad;
-    Tc q[C * kD];
+    static constexpr int kPad = Cfg<Tc>::kPad, kPadT = Cfg<Tc>::kPadT;
+    static constexpr int kQ = D1P + kPad, kD = D1P + kPadT, kN = 64 * NT + kPadT, kP = C + kPad;
+    Tc q[C * kQ];
     Tc k[C * kD];
     Tc v[C * kN];
     Tc p[C * kP];
     float pw[2 * C + 4];  // w^|x| at C + x
+    float pm[2 * C + 4];  // the same, zero on the side that P leaves out
 };
 template <typename Tc, int D1P, int NT, int C>
 struct LdsState {  // no queries
-    static constexpr int kPad = Cfg<Tc>::kPad;
-    static constexpr int kD = D1P + kPad, kN = 64 * NT + kPad, kP = 0;
+    static constexpr int kPadT = Cfg<Tc>::kPadT;
+    static constexpr int kQ = 0, kD = D1P + kPadT, kN = 64 * NT + kPadT, kP = 0;
     Tc k[C * kD];
     Tc v[C * kN];
     float pw[2 * C + 4];
@@ -258,8 +259,8 @@ struct LdsState {  // no queries
 
 // STATE_ONLY: the state a segment leaves behind when it starts from zero -> seg[segment], for all but a sequence's last.
 // VEC: rows of q, k, v are whole aligned packs, rows of o whole aligned quads, and a chunk of any of them spans < 2^29 bytes.
-template <typename Ti, typename Tc, int D1P, int NT, int C, bool STATE_ONLY, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Args a) {
+template <typename Ti, typename Tc, int D1P, int NT, int C, bool STATE_ONLY, bool VEC, bool late>
+__device__ __forceinline__ void linear_attention_body(const Args &a, const Role &role, int n0, int head, int b, int segment) {
     using F = typename Cfg<Tc>::frag;
     using L = typename std::conditional<STATE_ONLY, LdsState<Tc, D1P, NT, C>, Lds<Tc, D1P, NT, C>>::type;
     constexpr int VE = Cfg<Tc>::kVe;
@@ -270,29 +271,15 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
     extern __shared__ __attribute__((aligned(16))) char smem[];
     L &lds = *reinterpret_cast<L *>(smem);
 
-    // workgroup -> (segment, sequence, head, role, tile): the tiles and roles of a head next to each other
-    unsigned id = blockIdx.x;
-    int role_tiles = 0;
-    for (int r = 0; r < a.roles; ++r) role_tiles += a.role[r].tiles;
-    int t = id % role_tiles;
-    id /= role_tiles;
-    const int head = id % a.heads;
-    id /= a.heads;
-    const int b = id % a.batch;
-    const int segment = id / a.batch;
-    int ri = 0;
-    while (t >= a.role[ri].tiles) t -= a.role[ri++].tiles;
-    const Role &role = a.role[ri];
-    const int n0 = t * NB;
-
     long long start, len;
     sequence_rows(a, b, start, len);
     const long long u0 = segment * a.seg_len, u1 = min(len, u0 + a.seg_len);  // in the order of traversal
     if (STATE_ONLY && u1 >= len) return;
     if (u0 >= u1 && (segment > 0 || !role.s_out)) return;  // an empty sequence still hands its state on
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
-    const int d1 = role.d1, d2 = role.d2, late = role.late;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, m = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same in all its lanes: branches on it are scalar
+    const int d1 = role.d1, d2 = role.d2;
     const float log2w = a.log2_decay[head], read = role.read, write = role.write, pscale = role.pscale;
     const size_t bh = static_cast<size_t>(b) * a.heads + head;
     const long long base = a.offsets ? 0 : b;  // packed rows have no sequence stride
@@ -304,7 +291,11 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
     const int osize = partial ? 4 : static_cast<int>(sizeof(Ti));
     char *o = static_cast<char *>(role.o) + (base * role.os[0] + start * ot + head * role.os[2] + n0) * osize;
 
-    for (int x = tid; x <= 2 * C; x += kThreads) lds.pw[x] = power(log2w, static_cast<float>(x < C ? C - x : x - C));
+    for (int x = tid; x <= 2 * C; x += kThreads) {
+        const float w = power(log2w, static_cast<float>(x < C ? C - x : x - C));
+        lds.pw[x] = w;
+        if constexpr (!STATE_ONLY) lds.pm[x] = (late ? x <= C : x >= C) ? w : 0.0f;
+    }
 
     // the state: lane holds rows 16 dt + 4g + r, column n0 + 16 (NT wave + nt) + m
     f32x4 S[DT * NT];
@@ -379,24 +370,36 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
 #pragma unroll
         for (int x = 0; x < QV; ++x) {
             to_lds(lds.k + (qrow + x * QROWS) * L::kD + qcol, rk[x]);
-            if constexpr (!STATE_ONLY) to_lds(lds.q + (qrow + x * QROWS) * L::kD + qcol, rq[x]);
+            if constexpr (!STATE_ONLY) to_lds(lds.q + (qrow + x * QROWS) * L::kQ + qcol, rq[x]);
         }
 #pragma unroll
         for (int x = 0; x < VV; ++x) to_lds(lds.v + (vrow + x * VROWS) * L::kN + vcol, rv[x]);
     };
     auto size_at = [&](long long u) { return static_cast<int>(min(static_cast<long long>(C), u1 - u)); };
 
-    const Decay whole = decay_over(log2w, C);
+    // S holds the state times w^-owing
+    int owing = 0;
+    float owed = 1.0f;
+    auto settle_debt = [&]() {
+        const Decay w = decay_over(log2w, owing);
+#pragma unroll
+        for (int i = 0; i < DT * NT; ++i) S[i] = S[i] * w.hi + S[i] * w.lo;
+        owing = 0;
+        owed = 1.0f;
+    };
+
     if (u0 < u1) {
         fetch(u0, size_at(u0));
         commit();
     }
     __syncthreads();
+    settle(S);  // loaded here: in the loop the wait for it would be one for the rows on their way, too
 
     for (long long u = u0; u < u1; u += C) {
         const int size = size_at(u);
         const bool more = u + C < u1;
-        if (more) fetch(u + C, size_at(u + C));
+        if constexpr (STATE_ONLY)
+            if (more) fetch(u + C, size_at(u + C));
 
         const float *const pw_mirrored = lds.pw + C - (size - 1), *const pw_plain = lds.pw + C + 1;
         const float *const pw_read = late ? pw_mirrored : pw_plain, *const pw_write = late ? pw_plain : pw_mirrored;
@@ -417,20 +420,23 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
                 f32x4 p = {};
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) O[it * NT + nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                auto products = [&](auto with_p) {
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    const F qf = row_frag(lds.q + (16 * it + m) * L::kD + 32 * kb, g);
+                    for (int kb = 0; kb < KB; ++kb) {
+                        const F qf = row_frag(lds.q + (16 * it + m) * L::kQ + 32 * kb, g);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma(O[it * NT + nt], sf[kb][nt], qf);
-                    if (mine && (late ? jt >= it : jt <= it)) mma(p, kf[kb], qf);
-                }
+                        for (int nt = 0; nt < NT; ++nt) mma(O[it * NT + nt], sf[kb][nt], qf);
+                        if constexpr (decltype(with_p)::value) mma(p, kf[kb], qf);
+                    }
+                };
+                if (mine && (late ? jt >= it : jt <= it)) products(std::true_type());
+                else products(std::false_type());
                 if (mine && (late ? jt / 2 >= it / 2 : jt / 2 <= it / 2)) {
                     settle(p);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int gap = 16 * (it - jt) + m - 4 * g - r;
-                        const float w = pscale * lds.pw[C + gap];
-                        p[r] = (late ? -gap : gap) >= 0 ? p[r] * w : 0.0f;
+                        const float w = lds.pm[C + 16 * (it - jt) + m - 4 * g - r];
+                        p[r] = w != 0.0f ? p[r] * (w * pscale) : 0.0f;  // what is left out may be anything, NaN too
                     }
                     to_lds4(lds.p + (16 * it + m) * L::kP + 16 * jt + 4 * g, p);
                 }
@@ -438,11 +444,12 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
             settle(O);
 #pragma unroll
             for (int it = 0; it < IT; ++it) {
-                const float rd = read * pw_read[16 * it + m];
+                const float rd = read * owed * pw_read[16 * it + m];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) O[it * NT + nt] *= rd;
             }
             __syncthreads();
+            if (more) fetch(u + C, size_at(u + C));  // not before: their registers would be missing above
         }
 
         F vf[JB][NT];
@@ -484,17 +491,21 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
             }
         }
 
-        // S <- w^size S + K^T (weighted V), the weighted V in three bf16 parts (fp32: in one); rows behind the last are zeros
-        const Decay wc = size == C ? whole : decay_over(log2w, size);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) S[dt * NT + nt] = S[dt * NT + nt] * wc.hi + S[dt * NT + nt] * wc.lo;
+        // S <- w^size S + K^T (weighted V), the weighted V in three bf16 parts (fp32: in one); rows behind the last are zeros.
+        // What S is to be multiplied by is put off, V weighted the more, until it comes to 2^-16.
+        owing += size;
+        float weight = write;
+        if (log2w * static_cast<float>(owing) > -16.0f) {
+            owed = power(log2w, static_cast<float>(owing));
+            weight *= power(-log2w, static_cast<float>(owing));
+        } else {
+            settle_debt();
+        }
 #pragma unroll
         for (int jb = 0; jb < JB; ++jb) {
             float wj[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) wj[e] = write * pw_write[32 * jb + 16 * (e >> 2) + 4 * g + (e & 3)];
+            for (int e = 0; e < 8; ++e) wj[e] = weight * pw_write[32 * jb + 16 * (e >> 2) + 4 * g + (e & 3)];
             constexpr int PARTS = sizeof(Tc) == 2 ? 3 : 1, GROUP = 4;
             F part[PARTS][NT];
 #pragma unroll
@@ -533,6 +544,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
     if constexpr (STATE_ONLY) s_out = role.seg + (bh * (a.segments - 1) + segment) * d1 * d2;
     else if (role.s_out && u1 == len) s_out = role.s_out + bh * d1 * d2;
     if (s_out) {
+        settle_debt();
         int rows = d1, cols = d2;  // hidden from the compiler, which would keep 64 comparisons of the loads above for the stores
         asm volatile("" : "+s"(rows), "+s"(cols));
         const auto to = descriptor(s_out);
@@ -549,6 +561,26 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
                 }
             }
     }
+}
+
+template <typename Ti, typename Tc, int D1P, int NT, int C, bool STATE_ONLY, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Args a) {
+    // workgroup -> (segment, sequence, head, role, tile): the tiles and roles of a head next to each other
+    unsigned id = blockIdx.x;
+    unsigned role_tiles = 0;
+    for (int r = 0; r < a.roles; ++r) role_tiles += a.role[r].tiles;
+    int t = id % role_tiles;
+    id /= role_tiles;
+    const int head = id % a.heads;
+    id /= a.heads;
+    const int b = id % a.batch;
+    const int segment = id / a.batch;
+    int ri = 0;
+    while (t >= a.role[ri].tiles) t -= a.role[ri++].tiles;
+    const Role &role = a.role[ri];
+    const int n0 = t * 64 * NT;
+    if (role.late) linear_attention_body<Ti, Tc, D1P, NT, C, STATE_ONLY, VEC, true>(a, role, n0, head, b, segment);
+    else linear_attention_body<Ti, Tc, D1P, NT, C, STATE_ONLY, VEC, false>(a, role, n0, head, b, segment);
 }
 
 // D1P and NT by the host's rule; C by the type: 64 tokens, 32 where an element is four bytes or a row 256 of them (LDS)
