@@ -127,6 +127,7 @@ __device__ __forceinline__ void settle(f32x4 (&x)[N]) {
     if constexpr (N == 16) asm volatile("s_nop 7\n\ts_nop 7" : "+v"(x[8]), "+v"(x[9]), "+v"(x[10]), "+v"(x[11]), "+v"(x[12]), "+v"(x[13]), "+v"(x[14]), "+v"(x[15]));
     if constexpr (N == 4) settle(x[0], x[1], x[2], x[3]);
     if constexpr (N == 2) settle(x[0], x[1]);
+    if constexpr (N == 1) settle(x[0]);
 }
 
 // 8 contraction elements of one row: columns 4g .. 4g+3 and 16 + 4g .. of the 32 at p (p: the row's first of these 32)
@@ -405,41 +406,41 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
         const float *const pw_read = late ? pw_mirrored : pw_plain, *const pw_write = late ? pw_plain : pw_mirrored;
         f32x4 O[STATE_ONLY ? 2 : IT * NT];
         if constexpr (!STATE_ONLY) {
-            // P^T = K Q^T: wave w takes the keys of tile w % IT for every (4 / IT)-th tile of queries
+            // O^T = S^T Q^T, and P^T = K Q^T, of which wave w takes the keys of tile w % IT for every (4 / IT)-th tile of
+            // queries -- all of them: leaving out the tiles that the mask empties costs more in branches than it saves.
+            // The contraction is the outer loop: S becomes an operand 32 rows at a time.
+            constexpr int PT = IT * IT / 4;
             const int jt = wave % IT;
-            F sf[KB][NT], kf[KB];
+            f32x4 p[PT];
+#pragma unroll
+            for (int x = 0; x < PT; ++x) p[x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int x = 0; x < IT * NT; ++x) O[x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
-                kf[kb] = row_frag(lds.k + (16 * jt + m) * L::kD + 32 * kb, g);
+                F sf[NT];
+                const F kf = row_frag(lds.k + (16 * jt + m) * L::kD + 32 * kb, g);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) sf[kb][nt] = operand(S[2 * kb * NT + nt], S[(2 * kb + 1) * NT + nt], Tc());
-            }
+                for (int nt = 0; nt < NT; ++nt) sf[nt] = operand(S[2 * kb * NT + nt], S[(2 * kb + 1) * NT + nt], Tc());
 #pragma unroll
-            for (int it = 0; it < IT; ++it) {
-                const bool mine = it % (4 / IT) == wave / IT;
-                f32x4 p = {};
+                for (int it = 0; it < IT; ++it) {
+                    const F qf = row_frag(lds.q + (16 * it + m) * L::kQ + 32 * kb, g);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) O[it * NT + nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                auto products = [&](auto with_p) {
-#pragma unroll
-                    for (int kb = 0; kb < KB; ++kb) {
-                        const F qf = row_frag(lds.q + (16 * it + m) * L::kQ + 32 * kb, g);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma(O[it * NT + nt], sf[kb][nt], qf);
-                        if constexpr (decltype(with_p)::value) mma(p, kf[kb], qf);
-                    }
-                };
-                if (mine && (late ? jt >= it : jt <= it)) products(std::true_type());
-                else products(std::false_type());
-                if (mine && (late ? jt / 2 >= it / 2 : jt / 2 <= it / 2)) {
-                    settle(p);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float w = lds.pm[C + 16 * (it - jt) + m - 4 * g - r];
-                        p[r] = w != 0.0f ? p[r] * (w * pscale) : 0.0f;  // what is left out may be anything, NaN too
-                    }
-                    to_lds4(lds.p + (16 * it + m) * L::kP + 16 * jt + 4 * g, p);
+                    for (int nt = 0; nt < NT; ++nt) mma(O[it * NT + nt], sf[nt], qf);
+                    if constexpr (PT == IT) mma(p[it], kf, qf);
                 }
+                if constexpr (PT == 1) mma(p[0], kf, row_frag(lds.q + (16 * (wave / IT) + m) * L::kQ + 32 * kb, g));
+            }
+            settle(p);
+#pragma unroll
+            for (int x = 0; x < PT; ++x) {
+                const int it = PT == 1 ? wave / IT : x;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float w = lds.pm[C + 16 * (it - jt) + m - 4 * g - r];
+                    p[x][r] = w != 0.0f ? p[x][r] * (w * pscale) : 0.0f;  // what is left out may be anything, NaN too
+                }
+                to_lds4(lds.p + (16 * it + m) * L::kP + 16 * jt + 4 * g, p[x]);
             }
             settle(O);
 #pragma unroll
