@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libdsp_gpu.so")
@@ -67,13 +68,9 @@ EXPORTS = (
 EXCHANGE_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p)
 
 
-class LinearAttentionShape(C.Structure):
-    """dsp_gpu_linear_attention_shape"""
-    _fields_ = [("batch", C.c_size_t), ("n", C.c_size_t), ("rows", C.c_size_t),
-                ("heads", C.c_int), ("heads_q", C.c_int), ("heads_k", C.c_int), ("heads_v", C.c_int),
-                ("dim_k", C.c_int), ("dim_v", C.c_int), ("sample_type", C.c_int),
-                ("q_stride", C.c_longlong * 3), ("k_stride", C.c_longlong * 3), ("v_stride", C.c_longlong * 3),
-                ("o_stride", C.c_longlong * 3), ("offsets", C.c_void_p), ("lengths", C.c_void_p), ("zero_rest", C.c_int)]
+# dsp_gpu_linear_attention_shape, and stride arrays, as bytes: packing them takes a fraction of filling ctypes objects
+ATTENTION_SHAPE = struct.Struct("@3Q7i12q2Qi0q")
+STRIDES2, STRIDES3 = struct.Struct("@2q"), struct.Struct("@3q")
 
 
 class DspGpuError(RuntimeError):
@@ -119,12 +116,12 @@ def lib() -> C.CDLL:
         L.dsp_gpu_iir_multi_ex.restype = i
         L.dsp_gpu_biquad_swept.argtypes = [vp, vp, vp, sz, sz, sz, i, C.c_double, vp, i, vp]
         L.dsp_gpu_biquad_swept.restype = i
-        ll, d, shape = C.c_longlong, C.c_double, C.POINTER(LinearAttentionShape)
-        L.dsp_gpu_rotary.argtypes = [vp, vp, i, sz, sz, i, i, vp, vp, vp, i, i, vp, vp, ll, d, i, vp]
-        L.dsp_gpu_linear_attention_workspace.argtypes = [shape, i, C.POINTER(sz)]
-        L.dsp_gpu_linear_attention.argtypes = [vp, vp, vp, vp, shape, vp, d, vp, vp, vp, sz, vp]
-        L.dsp_gpu_linear_attention_backward.argtypes = [vp] * 7 + [shape, vp, d, vp, vp, vp, vp, sz, vp]
-        L.dsp_gpu_linear_attention_step.argtypes = [vp, vp, vp, vp, shape, vp, d, vp, vp, sz, vp]
+        ll, d, by = C.c_longlong, C.c_double, C.c_char_p  # by: packed bytes
+        L.dsp_gpu_rotary.argtypes = [vp, vp, i, sz, sz, i, i, by, by, by, i, i, vp, by, ll, d, i, vp]
+        L.dsp_gpu_linear_attention_workspace.argtypes = [by, i, C.POINTER(sz)]
+        L.dsp_gpu_linear_attention.argtypes = [vp, vp, vp, vp, by, by, d, vp, vp, vp, sz, vp]
+        L.dsp_gpu_linear_attention_backward.argtypes = [vp] * 7 + [by, by, d, vp, vp, vp, vp, sz, vp]
+        L.dsp_gpu_linear_attention_step.argtypes = [vp, vp, vp, vp, by, by, d, vp, vp, sz, vp]
         for name in ("dsp_gpu_rotary", "dsp_gpu_linear_attention_workspace", "dsp_gpu_linear_attention",
                      "dsp_gpu_linear_attention_backward", "dsp_gpu_linear_attention_step"):
             getattr(L, name).restype = i

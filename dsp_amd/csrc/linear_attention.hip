@@ -60,17 +60,23 @@ __device__ __forceinline__ bool row_taken(const Args &a, long long row) {
     return row % a.n < len;
 }
 
+struct Shared {
+    const float *part[3];
+    void *out[3];
+    int group[3], dim[3];
+};
+
 // part [row][heads][dim] fp32 -> out [row][heads / group][dim], heads of a group added in their order
 template <typename T>
-__global__ void __launch_bounds__(256) add_heads_kernel(const Args a, const float *part, T *out, int group, int dim) {
+__global__ void __launch_bounds__(256) add_heads_kernel(const Args a, const Shared g) {
     const long long row = blockIdx.x;
     if (!row_taken(a, row)) return;
-    const int heads = a.heads / group;
+    const int i = blockIdx.y, group = g.group[i], dim = g.dim[i], heads = a.heads / group;
     for (int e = threadIdx.x; e < heads * dim; e += 256) {
-        const float *p = part + (row * a.heads + (e / dim) * group) * dim + e % dim;
+        const float *p = g.part[i] + (row * a.heads + (e / dim) * group) * dim + e % dim;
         float sum = 0.0f;
         for (int h = 0; h < group; ++h) sum += p[static_cast<size_t>(h) * dim];
-        out[row * heads * dim + e] = static_cast<T>(sum);
+        static_cast<T *>(g.out[i])[row * heads * dim + e] = static_cast<T>(sum);
     }
 }
 
@@ -84,11 +90,18 @@ struct Rest {
     long long rows;
 };
 
-// zeros into the rows that no sequence holds (all samples are zero where their bits are)
+// zeros into the rows that no sequence holds (all samples are zero where their bits are): a thread looks at a row, and the
+// workgroup clears what its threads found
 __global__ void __launch_bounds__(256) zero_rest_kernel(const Args a, const Rest z) {
+    __shared__ int list[256], count;
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    const long long first = static_cast<long long>(blockIdx.x) * 256, mine = first + threadIdx.x;
+    if (mine < z.rows && !row_taken(a, mine)) list[atomicAdd(&count, 1)] = threadIdx.x;
+    __syncthreads();
     const int i = blockIdx.y;
-    for (long long row = blockIdx.x; row < z.rows; row += gridDim.x) {
-        if (row_taken(a, row)) continue;
+    for (int r = 0; r < count; ++r) {
+        const long long row = first + list[r];
         const long long at = a.offsets ? row * z.stride[i][1] : row / a.n * z.stride[i][0] + row % a.n * z.stride[i][1];
         for (int e = threadIdx.x; e < z.heads[i] * z.dim[i]; e += 256) {
             const long long to = at + e / z.dim[i] * z.stride[i][2] + e % z.dim[i];
@@ -99,7 +112,7 @@ __global__ void __launch_bounds__(256) zero_rest_kernel(const Args a, const Rest
 }
 
 int zero_rest(const Args &a, Rest &z, int count, hipStream_t s) {
-    zero_rest_kernel<<<dim3(static_cast<unsigned>(std::min<long long>(z.rows, 2048)), count), 256, 0, s>>>(a, z);
+    zero_rest_kernel<<<dim3(static_cast<unsigned>((z.rows + 255) / 256), count), 256, 0, s>>>(a, z);
     return check_launch("zero_rest_kernel");
 }
 
@@ -366,8 +379,10 @@ int run(const Shape &p, Args &a, const Plan &pl, char *seg_ws, hipStream_t s) {
     if (pl.segments > 1) {
         v.state_only = true;
         if (int rc = launch_kernel(a, v, p.sample_type, runs * tiles * (pl.segments - 1), s)) return rc;
-        join_segments_kernel<<<dim3(static_cast<unsigned>(runs * most), a.roles), 256, 0, s>>>(a);
-        if (int rc = check_launch("join_segments_kernel")) return rc;
+        if (pl.segments > kJoinSelf) {
+            join_segments_kernel<<<dim3(static_cast<unsigned>(runs * most), a.roles), 256, 0, s>>>(a);
+            if (int rc = check_launch("join_segments_kernel")) return rc;
+        }
         v.state_only = false;
     }
     return launch_kernel(a, v, p.sample_type, blocks, s);
@@ -444,8 +459,8 @@ int take_workspace(const char *who, size_t need, void *given, size_t given_bytes
 }
 
 template <typename T>
-int add_heads(const Args &a, const Shape &p, const float *part, void *out, int heads_x, int dim, hipStream_t s) {
-    add_heads_kernel<T><<<static_cast<unsigned>(total_rows(p)), 256, 0, s>>>(a, part, static_cast<T *>(out), p.heads / heads_x, dim);
+int add_heads(const Args &a, const Shape &p, const Shared &g, int count, hipStream_t s) {
+    add_heads_kernel<T><<<dim3(static_cast<unsigned>(total_rows(p)), count), 256, 0, s>>>(a, g);
     return check_launch("add_heads_kernel");
 }
 
@@ -603,11 +618,19 @@ int dsp_gpu_linear_attention_backward(const void *q, const void *k, const void *
         a.role[0] = role[2];
         if (int rc = run(p, a, bp.pl[2], ws, s)) return rc;
     }
+    Shared g{};
+    int count = 0;
     for (int i = 0; i < 3; ++i) {
         if (!part[i] || !rows || !p.n) continue;
-        int rc = p.sample_type == DSP_GPU_BF16 ? add_heads<__bf16>(a, p, part[i], grad[i], heads_x[i], dim[i], s)
-                 : p.sample_type == DSP_GPU_F16 ? add_heads<_Float16>(a, p, part[i], grad[i], heads_x[i], dim[i], s)
-                                                : add_heads<float>(a, p, part[i], grad[i], heads_x[i], dim[i], s);
+        g.part[count] = part[i];
+        g.out[count] = grad[i];
+        g.group[count] = p.heads / heads_x[i];
+        g.dim[count++] = dim[i];
+    }
+    if (count) {
+        const int rc = p.sample_type == DSP_GPU_BF16 ? add_heads<__bf16>(a, p, g, count, s)
+                       : p.sample_type == DSP_GPU_F16 ? add_heads<_Float16>(a, p, g, count, s)
+                                                      : add_heads<float>(a, p, g, count, s);
         if (rc) return rc;
     }
     if (!p.zero_rest || !(p.offsets || p.lengths) || !rows || !p.n) return DSP_GPU_OK;

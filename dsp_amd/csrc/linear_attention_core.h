@@ -37,6 +37,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256;
 constexpr int kMaxHeads = 256;
 constexpr int kMaxRoles = 3;
+// Up to so many segments a workgroup of the last pass joins the states before its own itself: that reads them
+// segments / 2 times instead of twice and a write, but saves a kernel that runs by itself.
+constexpr int kJoinSelf = 6;
 
 // One run of the operator: the forward pass has one, the backward pass three (gradients of q, k, v).
 struct Role {
@@ -300,19 +303,8 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
 
     // the state: lane holds rows 16 dt + 4g + r, column n0 + 16 (NT wave + nt) + m
     f32x4 S[DT * NT];
-    {
-        const float *s_in = nullptr;
-        int sd = d2, sn = 1;
-        if constexpr (!STATE_ONLY) {
-            if (segment > 0) {
-                s_in = role.seg + (bh * (a.segments - 1) + segment - 1) * d1 * d2;
-            } else if (role.s_in) {
-                s_in = role.s_in + bh * d1 * d2;
-                sd = role.s_in_d;
-                sn = role.s_in_n;
-            }
-        }
-        const auto from = descriptor(s_in);
+    auto load_state = [&](f32x4(&x)[DT * NT], const float *p, int sd, int sn) {
+        const auto from = descriptor(p);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -321,10 +313,28 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int d = 16 * dt + 4 * g + r;
-                    const unsigned at = s_in && d < d1 && n < d2 ? (d * sd + n * sn) * 4u : kOutside;
-                    S[dt * NT + nt][r] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0));
+                    const unsigned at = p && d < d1 && n < d2 ? (d * sd + n * sn) * 4u : kOutside;
+                    x[dt * NT + nt][r] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0));
                 }
             }
+    };
+    const float *const seg = role.seg + bh * (a.segments - 1) * d1 * d2;
+    const bool joined = a.segments > kJoinSelf;
+    if (STATE_ONLY) {
+        load_state(S, nullptr, 0, 0);
+    } else if (segment > 0 && joined) {
+        load_state(S, seg + static_cast<size_t>(segment - 1) * d1 * d2, d2, 1);
+    } else {
+        load_state(S, role.s_in ? role.s_in + bh * d1 * d2 : nullptr, role.s_in_d, role.s_in_n);
+        if (segment > 0) {  // the few segments before this one, joined on the spot
+            const Decay w = decay_over(log2w, a.seg_len);
+            for (int s = 0; s < segment; ++s) {
+                f32x4 local[DT * NT];
+                load_state(local, seg + static_cast<size_t>(s) * d1 * d2, d2, 1);
+#pragma unroll
+                for (int i = 0; i < DT * NT; ++i) S[i] = S[i] * w.hi + (S[i] * w.lo + local[i]);
+            }
+        }
     }
 
     const int qrow = tid * VE / D1P, qcol = tid * VE % D1P, vrow = tid * VE / NB, vcol = tid * VE % NB;

@@ -360,6 +360,15 @@ def biquad_swept(x, fc, bandwidth: float, kind: str = "bandpass", state=None, ou
 
 
 # ---- sequence layers -------------------------------------------------------------------------------------------------
+# One token of a serving step is a few microseconds on the GPU: these calls keep what they do on the host as short.
+
+_SAMPLE_TYPES = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16} if torch is not None else {}
+_LAYOUTS = {"half": capi.ROTARY_HALF, "interleaved": capi.ROTARY_INTERLEAVED}
+
+
+# the handle of a device's current stream, without the Stream object around it (most of what asking for one costs)
+_raw_stream = getattr(getattr(torch, "_C", None), "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _bad(message):
@@ -369,18 +378,21 @@ def _bad(message):
 def _sample_type(x, what):
     if not _is_torch(x) or not x.is_cuda:
         raise _bad(f"{what} must be a torch tensor on the GPU")
-    types = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
-    if x.dtype not in types:
+    kind = _SAMPLE_TYPES.get(x.dtype)
+    if kind is None:
         raise _bad(f"{what}: expected float32, float16 or bfloat16, got {x.dtype}")
-    return types[x.dtype]
+    return kind
 
 
-def _strides(x, what, packed=False):
-    """(batch, token, head) strides of a [batch, n, heads, dim] (packed: [rows, heads, dim]) tensor; 0 for an axis of one."""
-    if x.shape[-1] > 1 and x.stride(-1) != 1 and x.numel():
+def _strides4(x, what):
+    """(batch, token, head) strides of a [batch, n, heads, dim] tensor; packed [rows, heads, dim] and one token a row
+    [n, heads, dim]: batch stride 0.  0 for an axis of one."""
+    st, sh = x.stride(), x.shape
+    if st[-1] != 1 and sh[-1] > 1 and x.numel():
         raise _bad(f"{what}: the last axis must be contiguous")
-    st = [0 if n <= 1 else s for n, s in zip(x.shape[:-1], x.stride()[:-1])]
-    return [0] + st if packed else st
+    if len(sh) == 3:
+        return 0, st[0] if sh[0] > 1 else 0, st[1] if sh[1] > 1 else 0
+    return st[0] if sh[0] > 1 else 0, st[1] if sh[1] > 1 else 0, st[2] if sh[2] > 1 else 0
 
 
 def _index(x, like, count, what):
@@ -388,7 +400,31 @@ def _index(x, like, count, what):
     if not (_is_torch(x) and x.device == like.device and x.dtype == torch.int64 and tuple(x.shape) == (count,)
             and x.is_contiguous()):
         raise _bad(f"{what} must be a contiguous int64 tensor of {count} entries on x's device")
-    return x.data_ptr() if count else None
+    return x.data_ptr()
+
+
+def _new(like, shape):
+    """A contiguous tensor of `like`'s type and device."""
+    return torch.empty_like(like) if shape == like.shape and like.is_contiguous() else like.new_empty(shape)
+
+
+def _same(t, like, shape, what):
+    """A sample tensor of `like`'s type and device."""
+    if not (_is_torch(t) and t.dtype == like.dtype and t.device == like.device and t.shape == shape):
+        raise _bad(f"{what} must be a {like.dtype} tensor {tuple(shape)} on {like.device}")
+    return t
+
+
+def _call(x, fn, *args):
+    """fn(*args, stream) with x's GPU current, on its current stream."""
+    index = x.device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(x.device):
+            rc = fn(*args, _raw_stream(index))
+    if rc != capi.OK:
+        capi.check(rc)
 
 
 def rotary(x, inv_freq, positions=None, position: int = 0, layout: str = "half", inverse: bool = False, gain: float = 1.0,
@@ -401,93 +437,91 @@ def rotary(x, inv_freq, positions=None, position: int = 0, layout: str = "half",
     kind = _sample_type(x, "x")
     if x.ndim not in (3, 4):
         raise _bad("x must be [batch, n, heads, dim] or [n, heads, dim]")
-    layouts = {"half": capi.ROTARY_HALF, "interleaved": capi.ROTARY_INTERLEAVED}
-    if layout not in layouts:
+    if layout not in _LAYOUTS:
         raise _bad(f"layout {layout!r}")
-    inv_freq = np.ascontiguousarray(inv_freq, dtype=np.float64)
-    if inv_freq.ndim != 1:
+    freq = np.ascontiguousarray(inv_freq, dtype=np.float64)
+    if freq.ndim != 1:
         raise _bad("inv_freq must be one-dimensional")
-    y = torch.empty_like(x, memory_format=torch.contiguous_format) if out is None else out
-    if not _is_torch(y) or y.device != x.device or y.dtype != x.dtype or y.shape != x.shape:
-        raise _bad("out must have x's shape and type, on x's device")
-    x4, y4 = (x, y) if x.ndim == 4 else (x[None], y[None])
-    batch, n, heads, dim = x4.shape
-    ppos = pstride = None
+    y = _new(x, x.shape) if out is None else _same(out, x, x.shape, "out")
+    batch, n, heads, dim = x.shape if x.ndim == 4 else (1, *x.shape)
+    ppos, pstride = None, None
     if positions is not None:
         if not (_is_torch(positions) and positions.device == x.device and positions.dtype == torch.int64
                 and tuple(positions.shape) in ((batch, n), (n,))):
             raise _bad("positions must be int64 [batch, n] or [n] on x's device")
-        p2 = positions.expand(batch, n)
-        pstride = (C.c_longlong * 2)(*[0 if c <= 1 else s for c, s in zip(p2.shape, p2.stride())])
-        ppos = positions.data_ptr() if x.numel() else None
-    xs, ys = (C.c_longlong * 3)(*_strides(x4, "x")), (C.c_longlong * 3)(*_strides(y4, "out"))
-    with _on_device(x):
-        capi.check(capi.lib().dsp_gpu_rotary(x.data_ptr(), y.data_ptr(), kind, batch, n, heads, dim, xs, ys,
-                                             inv_freq.ctypes.data, 2 * inv_freq.size, layouts[layout], ppos, pstride,
-                                             int(position), float(gain), capi.INVERSE if inverse else capi.FORWARD,
-                                             _stream_of(x)))
+        st = positions.stride()
+        pstride = capi.STRIDES2.pack(st[0] if len(st) == 2 and batch > 1 else 0, st[-1] if n > 1 else 0)
+        ppos = positions.data_ptr()
+    _call(x, capi.lib().dsp_gpu_rotary, x.data_ptr(), y.data_ptr(), kind, batch, n, heads, dim,
+          capi.STRIDES3.pack(*_strides4(x, "x")), capi.STRIDES3.pack(*_strides4(y, "out")), freq.tobytes(), 2 * freq.size,
+          _LAYOUTS[layout], ppos, pstride, position, gain, capi.INVERSE if inverse else capi.FORWARD)
     return y
 
 
-def _attention_shape(q, k, v, log_decay, lengths, offsets, max_length, step=False):
-    """-> (shape, packed, log_decay, state shape); checks everything the C call cannot see."""
-    kind = _sample_type(q, "q")
-    for t, what in ((k, "k"), (v, "v")):
-        if _sample_type(t, what) != kind or t.device != q.device:
-            raise _bad(f"{what} must have q's type and device")
-    packed = offsets is not None
-    axes = 3 if packed or step else 4
-    if not (q.ndim == k.ndim == v.ndim == axes):
-        raise _bad("q, k and v must be " + ("[batch, heads, dim]" if step else "[rows, heads, dim] with offsets"
-                                            if packed else "[batch, n, heads, dim]"))
-    lead = q.shape[:axes - 2]
-    if k.shape[:axes - 2] != lead or v.shape[:axes - 2] != lead or k.shape[-1] != q.shape[-1]:
-        raise _bad(f"shapes of q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not belong together")
-    log_decay = np.ascontiguousarray(log_decay, dtype=np.float64)
-    if log_decay.ndim != 1:
-        raise _bad("log_decay must be one-dimensional: one value a head")
-    p = capi.LinearAttentionShape()
-    p.heads, p.heads_q, p.heads_k, p.heads_v = log_decay.size, q.shape[-2], k.shape[-2], v.shape[-2]
-    p.dim_k, p.dim_v, p.sample_type = q.shape[-1], v.shape[-1], kind
-    if packed:
-        if lengths is not None:
-            raise _bad("offsets and lengths exclude each other")
-        if offsets.ndim != 1 or offsets.numel() < 1:
-            raise _bad("offsets must have batch + 1 entries")
-        p.batch, p.rows = offsets.numel() - 1, lead[0]
-        p.n = lead[0] if max_length is None else int(max_length)
-        p.offsets = _index(offsets, q, p.batch + 1, "offsets")
-    elif step:
-        p.batch, p.n = lead[0], 1
-    else:
-        p.batch, p.n = lead
-        if lengths is not None:
-            p.lengths = _index(lengths, q, p.batch, "lengths")
-    if not packed and max_length is not None:
-        raise _bad("max_length goes with offsets")
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        st = _strides(t, name, packed)
-        getattr(p, name + "_stride")[:] = [st[0], 0, st[1]] if step else st
-    return p, packed, log_decay, (p.batch, p.heads, p.dim_k, p.dim_v)
+class _Attention:
+    """The checked arguments of a linear-attention call, and the C struct of them as bytes."""
+    __slots__ = ("heads", "batch", "out_shape", "state_shape", "log_decay", "lead", "tail", "device")
 
+    def __init__(self, q, k, v, log_decay, lengths, offsets, max_length, axes):
+        kind = _sample_type(q, "q")
+        if not (_is_torch(k) and _is_torch(v) and k.dtype == q.dtype == v.dtype and k.device == q.device == v.device):
+            raise _bad("k and v must have q's type and device")
+        qs, ks, vs = q.shape, k.shape, v.shape
+        if offsets is not None:
+            axes = 3
+        if not len(qs) == len(ks) == len(vs) == axes or qs[:-2] != ks[:-2] or qs[:-2] != vs[:-2] or qs[-1] != ks[-1]:
+            raise _bad(f"shapes of q {tuple(qs)}, k {tuple(ks)}, v {tuple(vs)} do not belong together")
+        self.log_decay = np.ascontiguousarray(log_decay, dtype=np.float64)
+        if self.log_decay.ndim != 1:
+            raise _bad("log_decay must be one-dimensional: one value a head")
+        self.heads = self.log_decay.size
+        batch, n, rows, poffsets, plengths = qs[0], 1, 0, 0, 0
+        if offsets is not None:
+            if lengths is not None:
+                raise _bad("offsets and lengths exclude each other")
+            if not _is_torch(offsets) or offsets.ndim != 1 or offsets.numel() < 1:
+                raise _bad("offsets must have batch + 1 entries")
+            batch, rows = offsets.numel() - 1, qs[0]
+            n = rows if max_length is None else int(max_length)
+            if n < 0:
+                raise _bad(f"max_length {n}")
+            poffsets = _index(offsets, q, batch + 1, "offsets")
+        elif max_length is not None:
+            raise _bad("max_length goes with offsets")
+        elif axes == 4:
+            n = qs[1]
+            if lengths is not None:
+                plengths = _index(lengths, q, batch, "lengths")
+        sq, sk, sv = _strides4(q, "q"), _strides4(k, "k"), _strides4(v, "v")
+        if axes == 3 and offsets is None:  # one token a row: the rows are the sequences
+            sq, sk, sv = ((s[1], 0, s[2]) for s in (sq, sk, sv))
+        self.batch = batch
+        self.out_shape = (*qs[:-2], self.heads, vs[-1])
+        self.state_shape = (batch, self.heads, qs[-1], vs[-1])
+        self.lead = (batch, n, rows, self.heads, qs[-2], ks[-2], vs[-2], qs[-1], vs[-1], kind, *sq, *sk, *sv)
+        self.tail = (poffsets, plengths)
+        self.device = q.device
 
-def _state(t, like, shape, what):
-    if t is None:
-        return None
-    if not (_is_torch(t) and t.device == like.device and t.dtype == torch.float32 and tuple(t.shape) == shape and t.is_contiguous()):
-        raise _bad(f"{what} must be a contiguous float32 tensor {shape} on q's device")
-    return t.data_ptr()
+    def shape(self, o, what, zero_rest, step=False):
+        so = _strides4(o, what)
+        return capi.ATTENTION_SHAPE.pack(*self.lead, *((so[1], 0, so[2]) if step else so), *self.tail, zero_rest)
 
+    def state(self, t, what, shape=None):
+        if t is None:
+            return None
+        if not (_is_torch(t) and t.dtype == torch.float32 and t.device == self.device and t.is_contiguous()
+                and t.shape == (shape or self.state_shape)):
+            raise _bad(f"{what} must be a contiguous float32 tensor {shape or self.state_shape} on q's device")
+        return t.data_ptr()
 
-def _attention_workspace(p, backward, like):
-    """A tensor of the bytes the call needs, or None: torch's allocator keeps calls, streams and captured graphs apart."""
-    need = C.c_size_t(0)
-    capi.check(capi.lib().dsp_gpu_linear_attention_workspace(C.byref(p), int(backward), C.byref(need)))
-    return torch.empty(need.value, dtype=torch.uint8, device=like.device) if need.value else None
-
-
-def _ws_args(ws):
-    return (None, 0) if ws is None else (ws.data_ptr(), ws.numel())
+    def workspace(self, shape, backward):
+        """(tensor, pointer, bytes) of what the call needs: torch's allocator keeps calls, streams and captured graphs apart."""
+        need = C.c_size_t(0)
+        capi.check(capi.lib().dsp_gpu_linear_attention_workspace(shape, backward, C.byref(need)))
+        if not need.value:
+            return None, None, 0
+        t = torch.empty(need.value, dtype=torch.uint8, device=self.device)
+        return t, t.data_ptr(), need.value
 
 
 def linear_attention(q, k, v, log_decay, scale: float = 1.0, state=None, new_state=None, lengths=None, offsets=None,
@@ -498,21 +532,14 @@ def linear_attention(q, k, v, log_decay, scale: float = 1.0, state=None, new_sta
     offsets int64 [batch + 1] on the device (max_length: the longest sequence, else all rows); a padded one: lengths int64
     [batch].  state / new_state: float32 [batch, heads, dim_k, dim_v] before the first and after the last token (may be the
     same tensor).  Returns o [batch, n, heads, dim_v] (rows of no sequence: zeros, or what `out` held)."""
-    p, packed, log_decay, st_shape = _attention_shape(q, k, v, log_decay, lengths, offsets, max_length)
-    shape = tuple(q.shape[:-2]) + (p.heads, p.dim_v)
-    if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
-        p.zero_rest = 1
-    elif not (_is_torch(out) and out.device == q.device and out.dtype == q.dtype and tuple(out.shape) == shape):
-        raise _bad(f"out must be a {q.dtype} tensor {shape} on q's device")
-    p.o_stride[:] = _strides(out, "out", packed)
-    s_in, s_out = _state(state, q, st_shape, "state"), _state(new_state, q, st_shape, "new_state")
-    with _on_device(q):
-        ws = _attention_workspace(p, False, q)
-        capi.check(capi.lib().dsp_gpu_linear_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), C.byref(p),
-                                                       log_decay.ctypes.data, float(scale), s_in, s_out, *_ws_args(ws),
-                                                       _stream_of(q)))
-    return out
+    a = _Attention(q, k, v, log_decay, lengths, offsets, max_length, 4)
+    o = _new(v, a.out_shape) if out is None else _same(out, q, a.out_shape, "out")
+    shape = a.shape(o, "out", out is None)
+    s_in, s_out = a.state(state, "state"), a.state(new_state, "new_state")
+    ws, pws, nws = a.workspace(shape, 0)
+    _call(q, capi.lib().dsp_gpu_linear_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), shape,
+          a.log_decay.tobytes(), scale, s_in, s_out, pws, nws)
+    return o
 
 
 def linear_attention_backward(q, k, v, log_decay, dout, scale: float = 1.0, state=None, dnew_state=None, dstate=None,
@@ -520,21 +547,14 @@ def linear_attention_backward(q, k, v, log_decay, dout, scale: float = 1.0, stat
     """The gradients (dq, dk, dv) of linear_attention from dout and, where given, dnew_state, that of the state after the
     last token.  `state`: as in the forward call.  dstate: a float32 tensor that receives the gradient of `state`.  Gradients
     of heads that several share are summed in order; rows of no sequence get zeros.  log_decay has none."""
-    p, packed, log_decay, st_shape = _attention_shape(q, k, v, log_decay, lengths, offsets, max_length)
-    shape = tuple(q.shape[:-2]) + (p.heads, p.dim_v)
-    if not (_is_torch(dout) and dout.device == q.device and dout.dtype == q.dtype and tuple(dout.shape) == shape):
-        raise _bad(f"dout must be a {q.dtype} tensor {shape} on q's device")
-    p.o_stride[:] = _strides(dout, "dout", packed)
-    s_in, ds_out = _state(state, q, st_shape, "state"), _state(dnew_state, q, st_shape, "dnew_state")
-    ds_in = _state(dstate, q, st_shape, "dstate")
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
-    p.zero_rest = 1
-    with _on_device(q):
-        ws = _attention_workspace(p, True, q)
-        capi.check(capi.lib().dsp_gpu_linear_attention_backward(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), *(g.data_ptr() for g in grads), C.byref(p),
-            log_decay.ctypes.data, float(scale), s_in, ds_out, ds_in, *_ws_args(ws), _stream_of(q)))
-    return tuple(grads)
+    a = _Attention(q, k, v, log_decay, lengths, offsets, max_length, 4)
+    shape = a.shape(_same(dout, q, a.out_shape, "dout"), "dout", True)
+    s_in, ds_out, ds_in = a.state(state, "state"), a.state(dnew_state, "dnew_state"), a.state(dstate, "dstate")
+    dq, dk, dv = _new(q, q.shape), _new(k, k.shape), _new(v, v.shape)
+    ws, pws, nws = a.workspace(shape, 1)
+    _call(q, capi.lib().dsp_gpu_linear_attention_backward, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
+          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), shape, a.log_decay.tobytes(), scale, s_in, ds_out, ds_in, pws, nws)
+    return dq, dk, dv
 
 
 def linear_attention_step(q, k, v, log_decay, state, scale: float = 1.0, slots=None, out=None):
@@ -542,27 +562,18 @@ def linear_attention_step(q, k, v, log_decay, state, scale: float = 1.0, slots=N
     [batch, heads, dim_k, dim_v], updated in place -- or [n_slots, ...] with slots int64 [batch] on the device, row b working
     on state[slots[b]] (a slot outside the pool: the row is skipped; the same slot twice: in the order of the rows).
     Returns o [batch, heads, dim_v] (skipped rows: zeros)."""
-    p, _, log_decay, st_shape = _attention_shape(q, k, v, log_decay, None, None, None, step=True)
-    shape = (p.batch, p.heads, p.dim_v)
-    pslots, n_slots = None, 0
-    if slots is not None:
-        pslots = _index(slots, q, p.batch, "slots")
-        n_slots = state.shape[0] if _is_torch(state) and state.ndim else 0
-        st_shape = (n_slots,) + st_shape[1:]
-    if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
-    elif not (_is_torch(out) and out.device == q.device and out.dtype == q.dtype and tuple(out.shape) == shape):
-        raise _bad(f"out must be a {q.dtype} tensor {shape} on q's device")
-    so = _strides(out, "out")
-    p.o_stride[:] = [so[0], 0, so[1]]
+    a = _Attention(q, k, v, log_decay, None, None, None, 3)
     if state is None:
         raise _bad("state must be given: it is what the step updates")
-    ps = _state(state, q, st_shape, "state")
-    with _on_device(q):
-        capi.check(capi.lib().dsp_gpu_linear_attention_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), C.byref(p),
-                                                            log_decay.ctypes.data, float(scale), ps, pslots, n_slots,
-                                                            _stream_of(q)))
-    return out
+    o = _new(v, a.out_shape) if out is None else _same(out, q, a.out_shape, "out")
+    if slots is None:
+        pslots, n_slots, ps = None, 0, a.state(state, "state")
+    else:
+        n_slots = state.shape[0] if _is_torch(state) and state.ndim else 0
+        pslots, ps = _index(slots, q, a.batch, "slots"), a.state(state, "state", (n_slots, *a.state_shape[1:]))
+    _call(q, capi.lib().dsp_gpu_linear_attention_step, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+          a.shape(o, "out", False, True), a.log_decay.tobytes(), scale, ps, pslots, n_slots)
+    return o
 
 
 def fft_kernel_ms(x, out, inverse: bool, iters: int) -> float:
