@@ -176,6 +176,34 @@ __device__ __forceinline__ bf16x8 operand(const f32x4 &a, const f32x4 &b, __bf16
 }
 __device__ __forceinline__ f32x8 operand(const f32x4 &a, const f32x4 &b, float) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
+// part[0] + part[1] + part[2] = v w to 24 bits, two elements at a time
+template <int NT>
+__device__ __forceinline__ void split(bf16x8 (&part)[3][NT], int nt, const bf16x8 &v, const float (&w)[8]) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const u32x4 in = __builtin_bit_cast(u32x4, v);
+    u32x4 out[3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float x = __uint_as_float(in[i] << 16) * w[2 * i], y = __uint_as_float(in[i] & 0xffff0000u) * w[2 * i + 1];
+#pragma unroll
+        for (int s = 0; s < 3; ++s) {
+            const unsigned xy = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{x, y}), bf16x2));
+            out[s][i] = xy;
+            x -= __uint_as_float(xy << 16);
+            y -= __uint_as_float(xy & 0xffff0000u);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < 3; ++s) part[s][nt] = __builtin_bit_cast(bf16x8, out[s]);
+}
+template <int NT>
+__device__ __forceinline__ void split(f32x8 (&part)[1][NT], int nt, const f32x8 &v, const float (&w)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[0][nt][e] = v[e] * w[e];
+}
+
 // ---- global <-> registers ----------------------------------------------------------------------------------------------
 
 template <typename T, int N>
@@ -394,7 +422,13 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
     auto settle_debt = [&]() {
         const Decay w = decay_over(log2w, owing);
 #pragma unroll
-        for (int i = 0; i < DT * NT; ++i) S[i] = S[i] * w.hi + S[i] * w.lo;
+        for (int i = 0; i < DT * NT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float x = S[i][r];
+                x = fmaf(x, w.hi, x * w.lo);
+                S[i][r] = x;
+            }
         owing = 0;
         owed = 1.0f;
     };
@@ -506,12 +540,10 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
         // What S is to be multiplied by is put off, V weighted the more, until it comes to 2^-16.
         owing += size;
         float weight = write;
-        if (log2w * static_cast<float>(owing) > -16.0f) {
-            owed = power(log2w, static_cast<float>(owing));
-            weight *= power(-log2w, static_cast<float>(owing));
-        } else {
-            settle_debt();
-        }
+        const bool pay = log2w * static_cast<float>(owing) <= -16.0f;
+        if (__builtin_expect(pay, 0)) settle_debt();
+        owed = power(log2w, static_cast<float>(owing));
+        weight *= power(-log2w, static_cast<float>(owing));
 #pragma unroll
         for (int jb = 0; jb < JB; ++jb) {
             float wj[8];
@@ -521,15 +553,7 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
             F part[PARTS][NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float x = static_cast<float>(vf[jb][nt][e]) * wj[e];
-#pragma unroll
-                    for (int s = 0; s < PARTS; ++s) {
-                        part[s][nt][e] = static_cast<Tc>(x);
-                        x -= static_cast<float>(part[s][nt][e]);
-                    }
-                }
+                split(part, nt, vf[jb][nt], wj);
 #pragma unroll
             for (int d0 = 0; d0 < DT; d0 += GROUP) {  // four tiles of rows at a time: products that do not wait for each other
                 F kc[GROUP];
