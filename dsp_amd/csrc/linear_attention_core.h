@@ -273,20 +273,20 @@ template <typename Tc, int D1P, int NT, int C>
 struct Lds {
     static constexpr int kPad = Cfg<Tc>::kPad, kPadT = Cfg<Tc>::kPadT;
     static constexpr int kQ = D1P + kPad, kD = D1P + kPadT, kN = 64 * NT + kPadT, kP = C + kPad;
+    float pw[2 * C + 4];  // w^|x| at C + x; in front, where the offsets of paired reads reach
+    float pm[2 * C + 4];  // the same, zero on the side that P leaves out
     Tc q[C * kQ];
     Tc k[C * kD];
     Tc v[C * kN];
     Tc p[C * kP];
-    float pw[2 * C + 4];  // w^|x| at C + x
-    float pm[2 * C + 4];  // the same, zero on the side that P leaves out
 };
 template <typename Tc, int D1P, int NT, int C>
 struct LdsState {  // no queries
     static constexpr int kPadT = Cfg<Tc>::kPadT;
     static constexpr int kQ = 0, kD = D1P + kPadT, kN = 64 * NT + kPadT, kP = 0;
+    float pw[2 * C + 4];
     Tc k[C * kD];
     Tc v[C * kN];
-    float pw[2 * C + 4];
 };
 
 // STATE_ONLY: the state a segment leaves behind when it starts from zero -> seg[segment], for all but a sequence's last.
@@ -416,22 +416,12 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
     };
     auto size_at = [&](long long u) { return static_cast<int>(min(static_cast<long long>(C), u1 - u)); };
 
-    // S holds the state times w^-owing
+    // S holds the state times w^-owing.  It is paid when that comes to 2^16, every `period` tokens, and after the last one.
     int owing = 0;
     float owed = 1.0f;
-    auto settle_debt = [&]() {
-        const Decay w = decay_over(log2w, owing);
-#pragma unroll
-        for (int i = 0; i < DT * NT; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float x = S[i][r];
-                x = fmaf(x, w.hi, x * w.lo);
-                S[i][r] = x;
-            }
-        owing = 0;
-        owed = 1.0f;
-    };
+    const float chunks = ceilf(-16.0f / (log2w * C));
+    const int period = C * (chunks >= 1.0f ? static_cast<int>(fminf(chunks, 1048576.0f)) : 1);
+    const Decay due = decay_over(log2w, period), rest = u0 < u1 ? decay_over(log2w, (u1 - u0 - 1) % period + 1) : Decay{1.0f, 0.0f};
 
     if (u0 < u1) {
         fetch(u0, size_at(u0));
@@ -537,13 +527,22 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
         }
 
         // S <- w^size S + K^T (weighted V), the weighted V in three bf16 parts (fp32: in one); rows behind the last are zeros.
-        // What S is to be multiplied by is put off, V weighted the more, until it comes to 2^-16.
+        // What S is to be multiplied by is put off, V weighted the more.
         owing += size;
-        float weight = write;
-        const bool pay = log2w * static_cast<float>(owing) <= -16.0f;
-        if (__builtin_expect(pay, 0)) settle_debt();
+        if (__builtin_expect(owing == period || !more, 0)) {
+            const float hi = more ? due.hi : rest.hi, lo = more ? due.lo : rest.lo;
+#pragma unroll
+            for (int i = 0; i < DT * NT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {  // x hi + x lo in x's own register: the compiler would take another 64
+                    float x = S[i][r], t;
+                    asm("v_mul_f32 %1, %2, %0\n\tv_fma_f32 %0, %0, %3, %1" : "+v"(x), "=&v"(t) : "v"(lo), "v"(hi));
+                    S[i][r] = x;
+                }
+            owing = 0;
+        }
         owed = power(log2w, static_cast<float>(owing));
-        weight *= power(-log2w, static_cast<float>(owing));
+        const float weight = write * power(-log2w, static_cast<float>(owing));
 #pragma unroll
         for (int jb = 0; jb < JB; ++jb) {
             float wj[8];
@@ -579,7 +578,6 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
     if constexpr (STATE_ONLY) s_out = role.seg + (bh * (a.segments - 1) + segment) * d1 * d2;
     else if (role.s_out && u1 == len) s_out = role.s_out + bh * d1 * d2;
     if (s_out) {
-        settle_debt();
         int rows = d1, cols = d2;  // hidden from the compiler, which would keep 64 comparisons of the loads above for the stores
         asm volatile("" : "+s"(rows), "+s"(cols));
         const auto to = descriptor(s_out);
