@@ -14,29 +14,39 @@ namespace {
 // ---- segments -> states ------------------------------------------------------------------------------------------------
 
 // seg[s] holds what segment s leaves behind from a zero state; afterwards it holds the state that segment s + 1 starts from.
-// One thread an element of the state; the loads do not depend on the recurrence.
+// A thread has kJoin elements of the state, 256 apart; the loads do not depend on the recurrence.
+constexpr int kJoin = 4;
 __global__ void __launch_bounds__(256) join_segments_kernel(const Args a) {
     const Role &role = a.role[blockIdx.y];
-    const int count = role.d1 * role.d2, blocks = (count + 255) / 256;
-    const int bh = blockIdx.x / blocks, e = (blockIdx.x % blocks) * 256 + threadIdx.x;
-    if (bh >= a.batch * a.heads || e >= count) return;
+    const int count = role.d1 * role.d2, blocks = (count + 256 * kJoin - 1) / (256 * kJoin);
+    const int bh = blockIdx.x / blocks, e0 = (blockIdx.x % blocks) * 256 * kJoin + threadIdx.x;
+    if (bh >= a.batch * a.heads) return;
     long long start, len;
     sequence_rows(a, bh / a.heads, start, len);
-    const int full = static_cast<int>((len - 1) / a.seg_len);  // segments with another one behind them (len = 0: none)
-    if (len == 0 || full == 0) return;
-    float run = 0.0f;
-    if (role.s_in) run = role.s_in[static_cast<size_t>(bh) * count + (e / role.d2) * role.s_in_d + (e % role.d2) * role.s_in_n];
-    float *seg = role.seg + static_cast<size_t>(bh) * (a.segments - 1) * count + e;
+    const int full = len > 0 ? static_cast<int>((len - 1) / a.seg_len) : 0;  // segments with another one behind them
+    if (full == 0) return;
+    float run[kJoin];
+#pragma unroll
+    for (int j = 0; j < kJoin; ++j) {
+        const int e = e0 + 256 * j;
+        run[j] = role.s_in && e < count ? role.s_in[static_cast<size_t>(bh) * count + (e / role.d2) * role.s_in_d + (e % role.d2) * role.s_in_n] : 0.0f;
+    }
+    float *seg = role.seg + static_cast<size_t>(bh) * (a.segments - 1) * count + e0;
     const Decay w = decay_over(a.log2_decay[bh % a.heads], a.seg_len);
-    for (int s0 = 0; s0 < full; s0 += 8) {
-        float local[8];
+    for (int s0 = 0; s0 < full; s0 += 4) {
+        float local[4][kJoin];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) local[i] = s0 + i < full ? seg[static_cast<size_t>(s0 + i) * count] : 0.0f;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+            for (int j = 0; j < kJoin; ++j) local[i][j] = s0 + i < full && e0 + 256 * j < count ? seg[static_cast<size_t>(s0 + i) * count + 256 * j] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
             if (s0 + i >= full) break;
-            run = fmaf(run, w.hi, fmaf(run, w.lo, local[i]));
-            seg[static_cast<size_t>(s0 + i) * count] = run;
+#pragma unroll
+            for (int j = 0; j < kJoin; ++j) {
+                run[j] = fmaf(run[j], w.hi, fmaf(run[j], w.lo, local[i][j]));
+                if (e0 + 256 * j < count) seg[static_cast<size_t>(s0 + i) * count + 256 * j] = run[j];
+            }
         }
     }
 }
@@ -173,6 +183,22 @@ __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
             }
         }
     }
+    float kd[ROWS], qd[ROWS];
+    f32x4 vv;
+    auto operands = [&]() {
+        const T *q = static_cast<const T *>(a.q) + b * a.qs[0] + (head / a.q_group) * a.qs[1];
+        const T *k = static_cast<const T *>(a.k) + b * a.ks[0] + (head / a.k_group) * a.ks[1];
+        const T *v = static_cast<const T *>(a.v) + b * a.vs[0] + (head / a.v_group) * a.vs[1] + n0;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int d = ry + 16 * i;
+            kd[i] = d < a.d1 ? static_cast<float>(k[d]) : 0.0f;
+            qd[i] = d < a.d1 ? static_cast<float>(q[d]) : 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) vv[c] = n0 + c < a.d2 ? static_cast<float>(v[c]) : 0.0f;
+    };
+    operands();  // on their way while the slots are looked through
     bool again = false;
     if (a.slots) {
         if (tid == 0) {
@@ -190,19 +216,11 @@ __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
         again = more != 0;
     }
     for (;;) {
-        const T *q = static_cast<const T *>(a.q) + b * a.qs[0] + (head / a.q_group) * a.qs[1];
-        const T *k = static_cast<const T *>(a.k) + b * a.ks[0] + (head / a.k_group) * a.ks[1];
-        const T *v = static_cast<const T *>(a.v) + b * a.vs[0] + (head / a.v_group) * a.vs[1] + n0;
-        f32x4 vv, acc = {};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) vv[c] = n0 + c < a.d2 ? static_cast<float>(v[c]) : 0.0f;
+        f32x4 acc = {};
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-            const int d = ry + 16 * i;
-            if (d < a.d1) {
-                s[i] = s[i] * w + (s[i] * w_lo + static_cast<float>(k[d]) * vv);
-                acc += static_cast<float>(q[d]) * s[i];
-            }
+            s[i] = s[i] * w + (s[i] * w_lo + kd[i] * vv);
+            acc += qd[i] * s[i];
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -220,6 +238,7 @@ __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
         for (++b; b < a.batch; ++b)
             if (a.slots[b] == slot) break;
         if (b >= a.batch) break;
+        operands();
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
@@ -298,13 +317,15 @@ struct Plan {
 };
 
 constexpr long long kSlots = 512;     // workgroups the chip runs at once: two on each of 256 CUs
-constexpr long long kLeast = 256;     // tokens of a segment at least: a state is written and read for each
+// Tokens of a segment at least: a state is written and read for each.  (2 x 1000 tokens of 12 heads, backward: 65 us; 256:
+// 89 us.  1 x 600 of 4 heads: 33 us; 256: 45 us, 64: 30 us, but 8 x 2048 of 16 heads 2 % slower.)
+constexpr long long kLeast = 128;
 
 // How the work of `roles` runs over batch * heads sequences is spread.  A workgroup that owns 128 columns reads q and k half
 // as often as two that own 64.  Where the runs do not fill the chip the time axis is cut into segments, which costs a
 // second pass over k and v (about kAgain of the first): dense batches take the number of segments with the least
-// ceil(workgroups / slots) * tokens of a segment; of ragged ones only the sum of the lengths is known, and the segments
-// are such that it makes about three rounds of half-filled slots.
+// ceil(workgroups / slots) * tokens of a segment; of packed ones only the sum of the lengths is known, and a segment is
+// its share of a slot (20,011 tokens of 16 heads in 16 sequences: 208 us; half of it 225 us, a third 237 us).
 Plan make_plan(const Shape &p, int d1, const int *d2, int roles) {
     Plan pl{};
     pl.d1p = d1 <= 64 ? 64 : d1 <= 128 ? 128 : 256;
@@ -320,7 +341,7 @@ Plan make_plan(const Shape &p, int d1, const int *d2, int roles) {
     if (n >= 2 * kLeast) {
         constexpr double kAgain = 0.4;
         if (p.offsets) {
-            pl.seg_len = std::min(pl.seg_len, std::max(kLeast, up(static_cast<long long>(p.rows) * groups / (kSlots * 3 / 2))));
+            pl.seg_len = std::min(pl.seg_len, std::max(kLeast, up(static_cast<long long>(p.rows) * groups / kSlots)));
         } else {
             double best = 0.0;
             for (long long s = 1; s <= 64 && s <= n / kLeast; ++s) {
@@ -371,7 +392,7 @@ int run(const Shape &p, Args &a, const Plan &pl, char *seg_ws, hipStream_t s) {
         x.tiles = (x.d2 + 64 * pl.nt - 1) / (64 * pl.nt);
         x.seg = pl.segments > 1 ? reinterpret_cast<float *>(seg_ws + r * segment_bytes(p, pl)) : nullptr;
         tiles += x.tiles;
-        most = std::max<size_t>(most, (static_cast<size_t>(x.d1) * x.d2 + 255) / 256);
+        most = std::max<size_t>(most, (static_cast<size_t>(x.d1) * x.d2 + 256 * kJoin - 1) / (256 * kJoin));
         v.vec = v.vec && x.vec;
     }
     const size_t runs = p.batch * p.heads, blocks = runs * tiles * pl.segments;
@@ -480,7 +501,7 @@ int dsp_gpu_linear_attention_workspace(const dsp_gpu_linear_attention_shape *sha
     if (!shape || !bytes) return fail(DSP_GPU_EINVAL, "%s: null argument", who);
     if (int rc = check_shape(who, *shape)) return rc;
     *bytes = 0;
-    if (shape->batch == 0 || shape->n == 0 || (shape->offsets && shape->rows == 0)) return DSP_GPU_OK;
+    if (shape->batch == 0 || total_rows(*shape) == 0) return DSP_GPU_OK;
     if (backward) {
         *bytes = backward_plan(*shape).total;
     } else {
@@ -501,9 +522,9 @@ int dsp_gpu_linear_attention(const void *q, const void *k, const void *v, void *
     if (int rc = check_decay(who, log_decay, p.heads, scale, a.log2_decay)) return rc;
     if (p.batch == 0) return DSP_GPU_OK;
     const size_t rows = total_rows(p);
-    if (rows && p.n && (!q || !k || !v || !o)) return fail(DSP_GPU_EINVAL, "%s: null buffer", who);
+    if (rows && (!q || !k || !v || !o)) return fail(DSP_GPU_EINVAL, "%s: null buffer", who);
     const size_t size = sample_bytes(p.sample_type), sb = state_bytes(p);
-    if (rows && p.n) {
+    if (rows) {
         const size_t batch = p.offsets ? 1 : p.batch, n = p.offsets ? p.rows : p.n;
         if (!rows_distinct(p.o_stride, batch, n, p.heads, p.dim_v)) return fail(DSP_GPU_EINVAL, "%s: rows of o overlap one another", who);
         const Range ro{static_cast<const char *>(o), extent(p.o_stride, batch, n, p.heads, p.dim_v, size)};
@@ -519,7 +540,7 @@ int dsp_gpu_linear_attention(const void *q, const void *k, const void *v, void *
     hipStream_t s = static_cast<hipStream_t>(stream);
     const Plan pl = make_plan(p, p.dim_k, &p.dim_v, 1);
     char *ws = nullptr;
-    if (int rc = take_workspace(who, rows && p.n ? segment_bytes(p, pl) : 0, workspace, workspace_bytes, s, &ws)) return rc;
+    if (int rc = take_workspace(who, rows ? segment_bytes(p, pl) : 0, workspace, workspace_bytes, s, &ws)) return rc;
     a.roles = 1;
     Role &r = a.role[0];
     fill_role(r, p, {q, p.q_stride, p.heads_q, p.dim_k}, {k, p.k_stride, p.heads_k, p.dim_k}, {v, p.v_stride, p.heads_v, p.dim_v}, o, p.o_stride, false);
@@ -530,7 +551,7 @@ int dsp_gpu_linear_attention(const void *q, const void *k, const void *v, void *
     r.s_in_n = 1;
     r.s_out = state_out;
     if (int rc = run(p, a, pl, ws, s)) return rc;
-    if (!p.zero_rest || !(p.offsets || p.lengths) || !rows || !p.n) return DSP_GPU_OK;
+    if (!p.zero_rest || !(p.offsets || p.lengths) || !rows) return DSP_GPU_OK;
     Rest z{};
     z.p[0] = o;
     set_strides(z.stride[0], p.o_stride);
@@ -553,9 +574,9 @@ int dsp_gpu_linear_attention_backward(const void *q, const void *k, const void *
     if (int rc = check_decay(who, log_decay, p.heads, scale, a.log2_decay)) return rc;
     if (p.batch == 0) return DSP_GPU_OK;
     const size_t rows = total_rows(p), size = sample_bytes(p.sample_type), sb = state_bytes(p);
-    if (rows && p.n && (!q || !k || !v || !dout || !dq || !dk || !dv)) return fail(DSP_GPU_EINVAL, "%s: null buffer", who);
+    if (rows && (!q || !k || !v || !dout || !dq || !dk || !dv)) return fail(DSP_GPU_EINVAL, "%s: null buffer", who);
     if (rows > 0x7fffffffu) return fail(DSP_GPU_EINVAL, "%s: %zu rows", who, rows);
-    if (rows && p.n) {
+    if (rows) {
         const size_t batch = p.offsets ? 1 : p.batch, n = p.offsets ? p.rows : p.n;
         const Range out[4] = {{static_cast<const char *>(dq), rows * p.heads_q * p.dim_k * size},
                               {static_cast<const char *>(dk), rows * p.heads_k * p.dim_k * size},
@@ -579,7 +600,7 @@ int dsp_gpu_linear_attention_backward(const void *q, const void *k, const void *
     hipStream_t s = static_cast<hipStream_t>(stream);
     const BackwardPlan bp = backward_plan(p);
     char *ws = nullptr;
-    if (int rc = take_workspace(who, rows && p.n ? bp.total : 0, workspace, workspace_bytes, s, &ws)) return rc;
+    if (int rc = take_workspace(who, rows ? bp.total : 0, workspace, workspace_bytes, s, &ws)) return rc;
 
     const Tensor tq{q, p.q_stride, p.heads_q, p.dim_k}, tk{k, p.k_stride, p.heads_k, p.dim_k}, tv{v, p.v_stride, p.heads_v, p.dim_v},
         tdo{dout, p.o_stride, p.heads, p.dim_v};
@@ -621,7 +642,7 @@ int dsp_gpu_linear_attention_backward(const void *q, const void *k, const void *
     Shared g{};
     int count = 0;
     for (int i = 0; i < 3; ++i) {
-        if (!part[i] || !rows || !p.n) continue;
+        if (!part[i] || !rows) continue;
         g.part[count] = part[i];
         g.out[count] = grad[i];
         g.group[count] = p.heads / heads_x[i];
@@ -633,7 +654,7 @@ int dsp_gpu_linear_attention_backward(const void *q, const void *k, const void *
                                                       : add_heads<float>(a, p, g, count, s);
         if (rc) return rc;
     }
-    if (!p.zero_rest || !(p.offsets || p.lengths) || !rows || !p.n) return DSP_GPU_OK;
+    if (!p.zero_rest || !(p.offsets || p.lengths) || !rows) return DSP_GPU_OK;
     Rest z{};
     for (int i = 0; i < 3; ++i) {
         z.p[i] = grad[i];

@@ -433,8 +433,7 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
     for (long long u = u0; u < u1; u += C) {
         const int size = size_at(u);
         const bool more = u + C < u1;
-        if constexpr (STATE_ONLY)
-            if (more) fetch(u + C, size_at(u + C));
+        if (more) fetch(u + C, size_at(u + C));
 
         const float *const pw_mirrored = lds.pw + C - (size - 1), *const pw_plain = lds.pw + C + 1;
         const float *const pw_read = late ? pw_mirrored : pw_plain, *const pw_write = late ? pw_plain : pw_mirrored;
@@ -484,7 +483,6 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
                 for (int nt = 0; nt < NT; ++nt) O[it * NT + nt] *= rd;
             }
             __syncthreads();
-            if (more) fetch(u + C, size_at(u + C));  // not before: their registers would be missing above
         }
 
         F vf[JB][NT];

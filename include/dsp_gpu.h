@@ -289,7 +289,7 @@ int dsp_gpu_biquad_swept(const float *x, const float *fc, float *y, size_t chann
  *     (y0, y1) = gain * (x0 cos - x1 sin, x0 sin + x1 cos)      at the angle pos * inv_freq[i]
  * pair i being elements (i, i + rot_dim/2) -- DSP_GPU_ROTARY_HALF -- or (2i, 2i+1) -- DSP_GPU_ROTARY_INTERLEAVED.  Elements
  * from rot_dim on are copied.  DSP_GPU_INVERSE turns by the negative angle: the gradient of the forward call.  Angles are
- * formed and reduced in double (positions of any size), cos and sin in fp32, the result rounded once.
+ * formed and reduced in double (off by |pos inv_freq| 2^-52 at most), cos and sin in fp32, the result rounded once.
  * 2 <= rot_dim <= dim <= 1024, rot_dim even, rot_dim <= 256; inv_freq: rot_dim/2 finite doubles (radians a position;
  * dsp_amd/design.py rotary_frequencies, also for long contexts).  positions: device int64, element (b, t) at
  * b * position_stride[0] + t * position_stride[1] (strides >= 0, 0 = shared), or NULL: position + t.
