@@ -360,7 +360,8 @@ def biquad_swept(x, fc, bandwidth: float, kind: str = "bandpass", state=None, ou
 
 
 # ---- sequence layers -------------------------------------------------------------------------------------------------
-# One token of a serving step is a few microseconds on the GPU: these calls keep what they do on the host as short.
+# One token of a serving step is a few microseconds on the GPU: these calls keep what they do on the host short, too.  Like
+# every call here they are not recorded by autograd: gradients are calls of their own.
 
 _SAMPLE_TYPES = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16} if torch is not None else {}
 _LAYOUTS = {"half": capi.ROTARY_HALF, "interleaved": capi.ROTARY_INTERLEAVED}

@@ -293,7 +293,8 @@ int dsp_gpu_biquad_swept(const float *x, const float *fc, float *y, size_t chann
  * 2 <= rot_dim <= dim <= 1024, rot_dim even, rot_dim <= 256; inv_freq: rot_dim/2 finite doubles (radians a position;
  * dsp_amd/design.py rotary_frequencies, also for long contexts).  positions: device int64, element (b, t) at
  * b * position_stride[0] + t * position_stride[1] (strides >= 0, 0 = shared), or NULL: position + t.
- * x == y with the same strides is in place; other overlaps are refused (DSP_GPU_EINVAL).  Gradients with respect to
+ * x == y with the same strides is in place; otherwise the memory ranges (first to last element) of x and y must not meet
+ * (DSP_GPU_EINVAL).  Gradients with respect to
  * inv_freq and gain are not offered.
  */
 #define DSP_GPU_ROTARY_HALF 0
@@ -321,7 +322,7 @@ int dsp_gpu_rotary(const void *x, void *y, int sample_type, size_t batch, size_t
  * and joined.  bf16: products of bf16 operands (the weighted q k products and the state as read are rounded to bf16; what
  * the state adds up is not); F16 and F32 multiply in fp32.  A NaN or infinity in a token's v reaches the tokens of its
  * own chunk (up to 63 before it).  Outputs do not depend on anything but the inputs and the shape: repeated calls agree
- * bit for bit.
+ * bit for bit.  The memory ranges (first to last element) of what is written must not meet those of anything else.
  * workspace: dsp_gpu_linear_attention_workspace bytes, 16-byte aligned, used until the call's work is done; NULL: the
  * library's own per (device, stream), which grows -- not under capture, and not for two graphs that run at once.
  *

@@ -206,6 +206,9 @@ def test_nothing_from_nothing(ops, dev):
     assert torch.equal(ds, d1)
     ops.linear_attention(q, k, v, decays(2), new_state=end)
     assert (end == 0).all()
+    rows, none = torch.ones(5, 2, 16, dtype=torch.bfloat16, device=dev), torch.zeros(1, dtype=torch.int64, device=dev)
+    assert (ops.linear_attention(rows, rows, rows, decays(2), offsets=none) == 0).all()  # rows, but no sequence
+    assert all((x == 0).all() for x in ops.linear_attention_backward(rows, rows, rows, decays(2), rows, offsets=none))
 
 
 @pytest.mark.parametrize("kind", TYPES)
