@@ -141,6 +141,13 @@ __device__ __forceinline__ void settle(f32x4 (&x)[N]) {
     if constexpr (N == 1) settle(x[0]);
 }
 
+// adds 0 if all of a lane group's elements are finite, else NaN somewhere
+__device__ __forceinline__ void times_zero(f32x4 &acc, bf16x8 a) { mma(acc, a, bf16x8{}); }
+__device__ __forceinline__ void times_zero(f32x4 &acc, f32x8 a) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e & 3] += a[e] * 0.0f;
+}
+
 // 8 contraction elements of one row: columns 4g .. 4g+3 and 16 + 4g .. of the 32 at p (p: the row's first of these 32)
 __device__ __forceinline__ bf16x8 row_frag(const __bf16 *p, int g) {
     const bf16x4 a = *reinterpret_cast<const bf16x4 *>(p + 4 * g), b = *reinterpret_cast<const bf16x4 *>(p + 16 + 4 * g);
@@ -502,17 +509,42 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
         if constexpr (!STATE_ONLY) {
             char *const op = o + lowest(u, size) * ot * osize;
             const auto dout = descriptor(op);
+            // 0 * NaN is NaN: a product with P would carry what is not finite in V to tokens that P leaves it out for.
+            f32x4 none = {};
 #pragma unroll
-            for (int it = 0; it < IT; ++it) {
+            for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
-                for (int jb = 0; jb < JB; ++jb) {
-                    if (late ? jb < it / 2 : jb > it / 2) continue;
-                    const F pf = row_frag(lds.p + (16 * it + m) * L::kP + 32 * jb, g);
+                for (int nt = 0; nt < NT; ++nt) times_zero(none, vf[jb][nt]);
+            settle(none);
+            const bool finite = none[0] == 0.0f && none[1] == 0.0f && none[2] == 0.0f && none[3] == 0.0f;
+            if (__builtin_expect(__all(finite), 1)) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma(O[it * NT + nt], vf[jb][nt], pf);
+                for (int it = 0; it < IT; ++it) {
+#pragma unroll
+                    for (int jb = 0; jb < JB; ++jb) {
+                        if (late ? jb < it / 2 : jb > it / 2) continue;
+                        const F pf = row_frag(lds.p + (16 * it + m) * L::kP + 32 * jb, g);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma(O[it * NT + nt], vf[jb][nt], pf);
+                    }
+                }
+                settle(O);
+            } else {  // token by token, by those that see it
+#pragma unroll 1
+                for (int j = 0; j < C; ++j) {
+                    const Tc *const vj = lds.v + j * L::kN + 16 * NT * wave + 4 * g;
+#pragma unroll
+                    for (int it = 0; it < IT; ++it) {
+                        const int i = 16 * it + m;
+                        if (late ? j < i : j > i) continue;
+                        const float pij = static_cast<float>(lds.p[i * L::kP + j]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) O[it * NT + nt][r] += pij * static_cast<float>(vj[16 * nt + r]);
+                    }
                 }
             }
-            settle(O);
 #pragma unroll
             for (int it = 0; it < IT; ++it) {
 #pragma unroll

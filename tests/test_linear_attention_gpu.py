@@ -266,6 +266,53 @@ def test_masked_places_may_hold_anything(ops, dev):
     assert torch.equal(out[:, :40], want)
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+def test_what_is_not_finite_stays_where_it_belongs(ops, dev, kind, bad):
+    """One bad element of q, k, v or dout: the outputs that the recurrence carries it to are not finite, all others are as
+    near as ever -- earlier tokens of the same chunk among them, in either direction of time."""
+    b, n, h, dk, dv, at = 1, 150, 2, 48, 72, 70
+    clean = make(dev, TYPES[kind], b, n, h, h, h, h, dk, dv, seed=11)
+    ld, terms = [-0.05, -0.2], dk + dv + n
+    for which in range(4):
+        q, k, v, do, s0, d1 = (x.clone() for x in clean)
+        (q, k, v, do)[which][0, at, 1, 5] = bad
+        end, ds = torch.empty_like(s0), torch.empty_like(s0)
+        out = ops.linear_attention(q, k, v, ld, scale=0.3, state=s0, new_state=end)
+        grads = ops.linear_attention_backward(q, k, v, ld, do, scale=0.3, state=s0, dnew_state=d1, dstate=ds)
+        args = [ref.heads_of(x, h) for x in (q, k, v)]
+        pos = [ref.heads_of(x, h).abs() for x in clean[:3]]
+        do64, cdo = do.cpu().double(), clean[3].cpu().double().abs()
+        want = [*ref.forward(*args, ld, 0.3, s0), *ref.backward(*args, ld, 0.3, s0, do64, d1)]
+        total = [*ref.forward(*pos, ld, 0.3, s0.abs()), *ref.backward(*pos, ld, 0.3, s0.abs(), cdo, d1.abs())]
+        for i, (x, w, t) in enumerate(zip((out, end, *grads, ds), want, total)):
+            fine = torch.isfinite(w)
+            assert torch.equal(torch.isfinite(x.cpu()), fine), (which, i)
+            ref.near(x.cpu()[fine], w[fine], t[fine], terms, x.dtype, operands=i not in (1, 5))
+
+
+def test_offsets_past_32_bits(ops, dev):
+    """Rows 2^17 bytes apart, 5 GB in all: the last ones are reached as the first ones are."""
+    n, h, d = 40000, 1, 64
+    big = torch.zeros(n, 1 << 16, dtype=torch.bfloat16, device=dev)
+    g = torch.Generator().manual_seed(1)
+    small = [torch.randn(n, h, d, generator=g).to(torch.bfloat16).to(dev) for _ in range(3)]
+    views = [big[:, i * 128:i * 128 + d].unflatten(-1, (h, d)) for i in range(3)]
+    for x, y in zip(views, small):
+        x.copy_(y)
+    wide = torch.empty(n, 1 << 16, dtype=torch.bfloat16, device=dev)[:, :d].unflatten(-1, (h, d))
+    want = ops.linear_attention(*(x[None] for x in small), [-0.01])
+    got = ops.linear_attention(*(x[None] for x in views), [-0.01], out=wide[None])
+    assert torch.equal(got, want)
+    do = small[0][None]
+    for x, y in zip(ops.linear_attention_backward(*(x[None] for x in views), [-0.01], do), ops.linear_attention_backward(*(x[None] for x in small), [-0.01], do)):
+        assert torch.equal(x, y)
+    freq = 0.5 ** torch.arange(32, dtype=torch.float64).numpy()
+    assert torch.equal(ops.rotary(views[0], freq), ops.rotary(small[0], freq))
+    step = ops.linear_attention_step(views[0][-2:], views[1][-2:], views[2][-2:], [-0.1], torch.zeros(2, 1, d, d, device=dev))
+    assert torch.equal(step, ops.linear_attention_step(small[0][-2:], small[1][-2:], small[2][-2:], [-0.1], torch.zeros(2, 1, d, d, device=dev)))
+
+
 def test_differences(ops, dev):
     """The fp32 gradients along random directions against central differences of the forward call (64-bit sums of its fp32
     outputs: their errors, 2^-24 of about 100 terms, come in divided by the step 2^-4 -- the function is a cubic in the
