@@ -51,6 +51,11 @@ __global__ void __launch_bounds__(256) join_segments_kernel(const Args a) {
     }
 }
 
+__global__ void __launch_bounds__(256) copy_state_kernel(const float *from, float *to, size_t count) {
+    const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i < count) to[i] = from[i];
+}
+
 // ---- gradients of shared heads -----------------------------------------------------------------------------------------
 
 // Whether a sequence holds `row` (of [batch][n], or of the packed batch) -- what the kernel above wrote.
@@ -365,6 +370,11 @@ size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 size_t segment_bytes(const Shape &p, const Plan &pl) {
     return pl.segments > 1 ? align256(sizeof(float) * p.batch * p.heads * (pl.segments - 1) * p.dim_k * p.dim_v) : 0;
 }
+// Of a forward call: the segments' states, and room for the state before the first token where it lies in place: the last
+// segment writes the state after the last one while others may still read it.
+size_t forward_bytes(const Shape &p, const Plan &pl) {
+    return pl.segments > 1 ? segment_bytes(p, pl) + align256(sizeof(float) * p.batch * p.heads * p.dim_k * p.dim_v) : 0;
+}
 size_t total_rows(const Shape &p) { return p.offsets ? p.rows : p.batch * p.n; }
 size_t part_bytes(const Shape &p, int heads_x, int dim) {
     return heads_x < p.heads ? align256(sizeof(float) * total_rows(p) * p.heads * dim) : 0;
@@ -513,7 +523,7 @@ int dsp_gpu_linear_attention_workspace(const dsp_gpu_linear_attention_shape *sha
         *bytes = backward_plan(*shape).total;
     } else {
         const Plan pl = make_plan(*shape, shape->dim_k, &shape->dim_v, 1);
-        *bytes = segment_bytes(*shape, pl);
+        *bytes = forward_bytes(*shape, pl);
     }
     return DSP_GPU_OK;
 }
@@ -547,7 +557,7 @@ int dsp_gpu_linear_attention(const void *q, const void *k, const void *v, void *
     hipStream_t s = static_cast<hipStream_t>(stream);
     const Plan pl = make_plan(p, p.dim_k, &p.dim_v, 1);
     char *ws = nullptr;
-    if (int rc = take_workspace(who, rows ? segment_bytes(p, pl) : 0, workspace, workspace_bytes, s, &ws)) return rc;
+    if (int rc = take_workspace(who, rows ? forward_bytes(p, pl) : 0, workspace, workspace_bytes, s, &ws)) return rc;
     a.roles = 1;
     Role &r = a.role[0];
     fill_role(r, p, {q, p.q_stride, p.heads_q, p.dim_k}, {k, p.k_stride, p.heads_k, p.dim_k}, {v, p.v_stride, p.heads_v, p.dim_v}, o, p.o_stride, false);
@@ -557,6 +567,14 @@ int dsp_gpu_linear_attention(const void *q, const void *k, const void *v, void *
     r.s_in_d = p.dim_v;
     r.s_in_n = 1;
     r.s_out = state_out;
+    if (pl.segments > 1 && state_in && state_in == state_out) {
+        float *const before = reinterpret_cast<float *>(ws + segment_bytes(p, pl));
+        const size_t count = sb / sizeof(float), blocks = (count + 255) / 256;
+        if (blocks > 0x7fffffffu) return fail(DSP_GPU_EINVAL, "%s: %zu elements of state", who, count);
+        copy_state_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(state_in, before, count);
+        if (int rc = check_launch("copy_state_kernel")) return rc;
+        r.s_in = before;
+    }
     if (int rc = run(p, a, pl, ws, s)) return rc;
     if (!p.zero_rest || !(p.offsets || p.lengths) || !rows) return DSP_GPU_OK;
     Rest z{};

@@ -196,6 +196,21 @@ def test_states_carried_on(ops, dev, kind):
     check_forward(q, k, v, ld, 0.2, s0, torch.cat(parts, 1), state)
 
 
+@pytest.mark.parametrize("n", [600, 1300])
+def test_state_in_place_of_a_long_prompt(ops, dev, n):
+    """Cut in time, with the state after the last token where the one before the first was: bit for bit the call with two."""
+    q, k, v, _, s0, _ = make(dev, torch.bfloat16, 2, n, 3, 3, 3, 3, 64, 80)
+    ld, end, both = [-0.001, -0.05, 0.0], torch.empty_like(s0), s0.clone()
+    out = ops.linear_attention(q, k, v, ld, scale=0.2, state=s0, new_state=end)
+    assert torch.equal(ops.linear_attention(q, k, v, ld, scale=0.2, state=both, new_state=both), out)
+    assert torch.equal(both, end)
+    lengths = torch.tensor([n, 40], device=dev)
+    both = s0.clone()
+    ops.linear_attention(q, k, v, ld, scale=0.2, state=s0, new_state=end, lengths=lengths)
+    ops.linear_attention(q, k, v, ld, scale=0.2, state=both, new_state=both, lengths=lengths)
+    assert torch.equal(both, end)
+
+
 def test_nothing_from_nothing(ops, dev):
     """No tokens: gradients of nothing, and the state's gradient handed on."""
     q, k, v, do, s0, d1 = make(dev, torch.bfloat16, 2, 0, 2, 2, 2, 2, 16, 16)
