@@ -13,7 +13,7 @@ namespace {
 
 // ---- segments -> states ------------------------------------------------------------------------------------------------
 
-// seg[s] holds what segment s leaves behind from a zero state; afterwards it holds the state that segment s + 1 starts from.
+// The slot of segment s holds what it leaves behind from a zero state; afterwards, the state that segment s + 1 starts from.
 // A thread has kJoin elements of the state, 256 apart; the loads do not depend on the recurrence.
 constexpr int kJoin = 4;
 __global__ void __launch_bounds__(256) join_segments_kernel(const Args a) {
@@ -23,29 +23,31 @@ __global__ void __launch_bounds__(256) join_segments_kernel(const Args a) {
     if (bh >= a.batch * a.heads) return;
     long long start, len;
     sequence_rows(a, bh / a.heads, start, len);
-    const int full = len > 0 ? static_cast<int>((len - 1) / a.seg_len) : 0;  // segments with another one behind them
+    const int full = inner_segments(a, len);
     if (full == 0) return;
+    const Slots slots = slots_of(a, role.late, bh / a.heads, start, len);
     float run[kJoin];
 #pragma unroll
     for (int j = 0; j < kJoin; ++j) {
         const int e = e0 + 256 * j;
         run[j] = role.s_in && e < count ? role.s_in[static_cast<size_t>(bh) * count + (e / role.d2) * role.s_in_d + (e % role.d2) * role.s_in_n] : 0.0f;
     }
-    float *seg = role.seg + static_cast<size_t>(bh) * (a.segments - 1) * count + e0;
+    float *seg = role.seg + (static_cast<size_t>(bh % a.heads) * a.slots + slots.first) * count + e0;
+    const int step = slots.step * count;
     const Decay w = decay_over(a.log2_decay[bh % a.heads], a.seg_len);
-    for (int s0 = 0; s0 < full; s0 += 4) {
+    for (int s0 = 0; s0 < full; s0 += 4, seg += 4 * step) {
         float local[4][kJoin];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < kJoin; ++j) local[i][j] = s0 + i < full && e0 + 256 * j < count ? seg[static_cast<size_t>(s0 + i) * count + 256 * j] : 0.0f;
+            for (int j = 0; j < kJoin; ++j) local[i][j] = s0 + i < full && e0 + 256 * j < count ? seg[i * step + 256 * j] : 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (s0 + i >= full) break;
 #pragma unroll
             for (int j = 0; j < kJoin; ++j) {
                 run[j] = fmaf(run[j], w.hi, fmaf(run[j], w.lo, local[i][j]));
-                if (e0 + 256 * j < count) seg[static_cast<size_t>(s0 + i) * count + 256 * j] = run[j];
+                if (e0 + 256 * j < count) seg[i * step + 256 * j] = run[j];
             }
         }
     }
@@ -62,14 +64,8 @@ __global__ void __launch_bounds__(256) copy_state_kernel(const float *from, floa
 __device__ __forceinline__ bool row_taken(const Args &a, long long row) {
     if (a.batch == 0) return false;
     long long start, len;
-    if (a.offsets) {  // the last sequence that starts at or before it
-        int lo = 0, hi = a.batch - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (a.offsets[mid] <= row) lo = mid;
-            else hi = mid - 1;
-        }
-        sequence_rows(a, lo, start, len);
+    if (a.offsets) {
+        sequence_rows(a, sequence_at(a, row), start, len);
         return row >= start && row < start + len;
     }
     sequence_rows(a, static_cast<int>(row / a.n), start, len);
@@ -321,6 +317,7 @@ int check_shape(const char *who, const Shape &p) {
 struct Plan {
     int d1p, nt, segments;
     long long seg_len;
+    size_t slots;  // segments that leave a state to the next one, of all sequences together
 };
 
 constexpr long long kSlots = 512;     // workgroups the chip runs at once: two on each of 256 CUs
@@ -362,13 +359,14 @@ Plan make_plan(const Shape &p, int d1, const int *d2, int roles) {
         }
     }
     pl.segments = static_cast<int>(std::max<long long>(1, (n + pl.seg_len - 1) / pl.seg_len));
+    if (pl.segments > 1) pl.slots = p.offsets ? p.rows / static_cast<size_t>(pl.seg_len) : p.batch * (pl.segments - 1);
     return pl;
 }
 
 size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
 size_t segment_bytes(const Shape &p, const Plan &pl) {
-    return pl.segments > 1 ? align256(sizeof(float) * p.batch * p.heads * (pl.segments - 1) * p.dim_k * p.dim_v) : 0;
+    return align256(sizeof(float) * pl.slots * p.heads * p.dim_k * p.dim_v);
 }
 // Of a forward call: the segments' states, and room for the state before the first token where it lies in place: the last
 // segment writes the state after the last one while others may still read it.
@@ -397,6 +395,7 @@ int run(const Shape &p, Args &a, const Plan &pl, char *seg_ws, hipStream_t s) {
     a.lengths = p.lengths;
     a.segments = pl.segments;
     a.seg_len = pl.seg_len;
+    a.slots = static_cast<unsigned>(pl.slots);
     size_t tiles = 0, most = 0;
     Variant v{pl.d1p, pl.nt, true, false};
     for (int r = 0; r < a.roles; ++r) {
@@ -407,12 +406,12 @@ int run(const Shape &p, Args &a, const Plan &pl, char *seg_ws, hipStream_t s) {
         most = std::max<size_t>(most, (static_cast<size_t>(x.d1) * x.d2 + 256 * kJoin - 1) / (256 * kJoin));
         v.vec = v.vec && x.vec;
     }
-    const size_t runs = p.batch * p.heads, blocks = runs * tiles * pl.segments;
+    const size_t runs = p.batch * p.heads, inner = pl.slots * p.heads * tiles, blocks = inner + runs * tiles;
     if (runs == 0) return DSP_GPU_OK;
     if (blocks > 0x7fffffffu || runs * most > 0x7fffffffu) return fail(DSP_GPU_EINVAL, "linear attention: %zu workgroups", blocks);
     if (pl.segments > 1) {
         v.state_only = true;
-        if (int rc = launch_kernel(a, v, p.sample_type, runs * tiles * (pl.segments - 1), s)) return rc;
+        if (int rc = launch_kernel(a, v, p.sample_type, inner, s)) return rc;
         if (pl.segments > kJoinSelf) {
             join_segments_kernel<<<dim3(static_cast<unsigned>(runs * most), a.roles), 256, 0, s>>>(a);
             if (int rc = check_launch("join_segments_kernel")) return rc;

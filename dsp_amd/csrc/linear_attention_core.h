@@ -63,14 +63,15 @@ struct Role {
     const float *s_in;             // [sequence][head] blocks of d1 * d2, element (d, n) at d * s_in_d + n * s_in_n; or null
     int s_in_d, s_in_n;
     float *s_out;                  // [sequence][head][d1][d2] or null
-    float *seg;                    // [sequence * heads + head][segments - 1][d1][d2]: states between the segments
+    float *seg;                    // [head][slot][d1][d2]: states between the segments (Slots)
 };
 
 struct Args {
     Role role[kMaxRoles];
     int roles;
     int heads, batch;
-    int segments;
+    int segments;                  // of the longest sequence that there can be
+    unsigned slots;                // states between the segments, for each head
     long long seg_len;             // tokens of a segment, a multiple of the chunk
     long long n;                   // tokens of a sequence at most
     long long rows;                // rows of a packed batch
@@ -92,6 +93,34 @@ __device__ __forceinline__ void sequence_rows(const Args &a, int b, long long &s
         const long long l = a.lengths[b];
         len = l < 0 ? 0 : l < a.n ? l : a.n;
     }
+}
+
+// The last sequence of a packed batch that starts at or before `row` (or the first one).
+__device__ __forceinline__ int sequence_at(const Args &a, long long row) {
+    int lo = 0, hi = a.batch - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.offsets[mid] <= row) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Segments of a sequence with another one behind them: those that leave a state between the segments.
+__device__ __forceinline__ int inner_segments(const Args &a, long long len) {
+    return len > 0 ? static_cast<int>(static_cast<unsigned>(len - 1) / static_cast<unsigned>(a.seg_len)) : 0;
+}
+
+// Which slot holds the state that segment s of a sequence leaves behind: first + s * step.  A dense batch has segments - 1
+// slots for each sequence.  The inner segments of a packed one are seg_len rows each that no other has, so the numbers
+// (first row of it) / seg_len are all different and below rows / seg_len: that many slots, however the rows are dealt out.
+struct Slots {
+    int first, step;
+};
+__device__ __forceinline__ Slots slots_of(const Args &a, int late, int b, long long start, long long len) {
+    if (!a.offsets) return {b * (a.segments - 1), 1};
+    const unsigned l = static_cast<unsigned>(a.seg_len);
+    return late ? Slots{static_cast<int>(static_cast<unsigned>(start + len) / l) - 1, -1} : Slots{static_cast<int>(static_cast<unsigned>(start) / l), 1};
 }
 
 // w^n for n >= 0, from log2 w (-inf for w = 0: w^0 is still 1)
@@ -307,7 +336,7 @@ struct LdsState {  // no queries
 // STATE_ONLY: the state a segment leaves behind when it starts from zero -> seg[segment], for all but a sequence's last.
 // VEC: rows of q, k, v are whole aligned packs, rows of o whole aligned quads, and a chunk of any of them spans < 2^29 bytes.
 template <typename Ti, typename Tc, int D1P, int NT, int C, bool STATE_ONLY, bool VEC, bool late>
-__device__ __forceinline__ void linear_attention_body(const Args &a, const Role &role, int n0, int head, int b, int segment) {
+__device__ __forceinline__ void linear_attention_body(const Args &a, const Role &role, int n0, int head, int b, long long start, long long len, int segment, Slots slots) {
     using F = typename Cfg<Tc>::frag;
     using L = typename std::conditional<STATE_ONLY, LdsState<Tc, D1P, NT, C>, Lds<Tc, D1P, NT, C>>::type;
     constexpr int VE = Cfg<Tc>::kVe;
@@ -318,8 +347,6 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
     extern __shared__ __attribute__((aligned(16))) char smem[];
     L &lds = *reinterpret_cast<L *>(smem);
 
-    long long start, len;
-    sequence_rows(a, b, start, len);
     const long long u0 = segment * a.seg_len, u1 = min(len, u0 + a.seg_len);  // in the order of traversal
     if (STATE_ONLY && u1 >= len) return;
     if (u0 >= u1 && (segment > 0 || !role.s_out)) return;  // an empty sequence still hands its state on
@@ -365,19 +392,19 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
                 }
             }
     };
-    const float *const seg = role.seg + bh * (a.segments - 1) * d1 * d2;
+    auto seg = [&](int s) { return role.seg + (static_cast<size_t>(head) * a.slots + slots.first + s * slots.step) * d1 * d2; };
     const bool joined = a.segments > kJoinSelf;
     if (STATE_ONLY) {
         load_state(S, nullptr, 0, 0);
     } else if (segment > 0 && joined) {
-        load_state(S, seg + static_cast<size_t>(segment - 1) * d1 * d2, d2, 1);
+        load_state(S, seg(segment - 1), d2, 1);
     } else {
         load_state(S, role.s_in ? role.s_in + bh * d1 * d2 : nullptr, role.s_in_d, role.s_in_n);
         if (segment > 0) {  // the few segments before this one, joined on the spot
             const Decay w = decay_over(log2w, a.seg_len);
             for (int s = 0; s < segment; ++s) {
                 f32x4 local[DT * NT];
-                load_state(local, seg + static_cast<size_t>(s) * d1 * d2, d2, 1);
+                load_state(local, seg(s), d2, 1);
 #pragma unroll
                 for (int i = 0; i < DT * NT; ++i) S[i] = S[i] * w.hi + (S[i] * w.lo + local[i]);
             }
@@ -621,7 +648,7 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
     }
 
     float *s_out = nullptr;
-    if constexpr (STATE_ONLY) s_out = role.seg + (bh * (a.segments - 1) + segment) * d1 * d2;
+    if constexpr (STATE_ONLY) s_out = seg(segment);
     else if (role.s_out && u1 == len) s_out = role.s_out + bh * d1 * d2;
     if (s_out) {
         int rows = d1, cols = d2;  // hidden from the compiler, which would keep 64 comparisons of the loads above for the stores
@@ -644,7 +671,7 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
 
 template <typename Ti, typename Tc, int D1P, int NT, int C, bool STATE_ONLY, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Args a) {
-    // workgroup -> (segment, sequence, head, role, tile): the tiles and roles of a head next to each other
+    // workgroup -> (segment of a sequence, head, role, tile): the tiles and roles of a head next to each other
     unsigned id = blockIdx.x;
     unsigned role_tiles = 0;
     for (int r = 0; r < a.roles; ++r) role_tiles += a.role[r].tiles;
@@ -652,14 +679,35 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
     id /= role_tiles;
     const int head = id % a.heads;
     id /= a.heads;
-    const int b = id % a.batch;
-    const int segment = id / a.batch;
     int ri = 0;
     while (t >= a.role[ri].tiles) t -= a.role[ri++].tiles;
     const Role &role = a.role[ri];
     const int n0 = t * 64 * NT;
-    if (role.late) linear_attention_body<Ti, Tc, D1P, NT, C, STATE_ONLY, VEC, true>(a, role, n0, head, b, segment);
-    else linear_attention_body<Ti, Tc, D1P, NT, C, STATE_ONLY, VEC, false>(a, role, n0, head, b, segment);
+    int b, segment;
+    long long start, len;
+    Slots slots;
+    if (a.offsets && a.segments > 1) {  // the slots' segments first, then the last segment of every sequence
+        if (id < a.slots) {
+            // seg_len rows from one in [id, id + 1) * seg_len on hold the last row of that range, whatever the offsets are
+            b = sequence_at(a, (id + 1) * a.seg_len - 1);
+            sequence_rows(a, b, start, len);
+            slots = slots_of(a, role.late, b, start, len);
+            segment = (static_cast<int>(id) - slots.first) * slots.step;
+            if (segment < 0 || segment >= inner_segments(a, len)) return;  // no segment has this slot
+        } else {
+            b = id - a.slots;
+            sequence_rows(a, b, start, len);
+            slots = slots_of(a, role.late, b, start, len);
+            segment = inner_segments(a, len);
+        }
+    } else {
+        b = id % a.batch;
+        segment = id / a.batch;
+        sequence_rows(a, b, start, len);
+        slots = slots_of(a, role.late, b, start, len);
+    }
+    if (role.late) linear_attention_body<Ti, Tc, D1P, NT, C, STATE_ONLY, VEC, true>(a, role, n0, head, b, start, len, segment, slots);
+    else linear_attention_body<Ti, Tc, D1P, NT, C, STATE_ONLY, VEC, false>(a, role, n0, head, b, start, len, segment, slots);
 }
 
 // D1P and NT by the host's rule; C by the type: 64 tokens, 32 where an element is four bytes or a row 256 of them (LDS)

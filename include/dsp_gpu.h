@@ -312,7 +312,8 @@ int dsp_gpu_rotary(const void *x, void *y, int sample_type, size_t batch, size_t
  * reads head h / (heads / heads_q) of q, and so on.  1 <= heads <= 256, 1 <= dim_k, dim_v <= 256.
  * log_decay: heads doubles <= 0 (-inf: nothing is remembered).  It is a constant of the head: no gradient is offered.
  *   offsets   (device int64, batch + 1, may be NULL) a PACKED batch: sequence b is rows offsets[b] .. offsets[b+1] of
- *             `rows` rows, the batch strides are not used and n is the length of the longest sequence
+ *             `rows` rows, the batch strides are not used and n is the length of the longest sequence, or anything above
+ *             it.  Offsets do not decrease: rows that two sequences claim would be written by both
  *   lengths   (device int64, batch, may be NULL) a PADDED batch: only the first lengths[b] tokens of sequence b are read
  * Rows that belong to no sequence are not read, and not written either unless zero_rest asks for zeros there; values outside
  * the tensors are taken as the nearest inside, and tokens from n on are left out.
