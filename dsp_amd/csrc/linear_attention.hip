@@ -53,9 +53,24 @@ __global__ void __launch_bounds__(256) join_segments_kernel(const Args a) {
     }
 }
 
-__global__ void __launch_bounds__(256) copy_state_kernel(const float *from, float *to, size_t count) {
-    const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i < count) to[i] = from[i];
+// A state in place: where a sequence has several segments, others may still read the state before its first token when the
+// last one is done.  That one leaves its state in the slot of the segment before it, which nobody else reads any more (of the
+// columns that are its own), and this brings it to its place.
+__global__ void __launch_bounds__(256) copy_states_kernel(const Args a) {
+    const Role &role = a.role[0];
+    const int count = role.d1 * role.d2, blocks = (count + 256 * kJoin - 1) / (256 * kJoin);
+    const int bh = blockIdx.x / blocks, e0 = (blockIdx.x % blocks) * 256 * kJoin + threadIdx.x;
+    if (bh >= a.batch * a.heads) return;
+    long long start, len;
+    sequence_rows(a, bh / a.heads, start, len);
+    const int full = inner_segments(a, len);
+    if (full == 0) return;
+    const Slots slots = slots_of(a, role.late, bh / a.heads, start, len);
+    const float *from = role.seg + (static_cast<size_t>(bh % a.heads) * a.slots + slots.first + (full - 1) * slots.step) * count;
+    float *to = role.s_out + static_cast<size_t>(bh) * count;
+#pragma unroll
+    for (int j = 0; j < kJoin; ++j)
+        if (e0 + 256 * j < count) to[e0 + 256 * j] = from[e0 + 256 * j];
 }
 
 // ---- gradients of shared heads -----------------------------------------------------------------------------------------
@@ -368,11 +383,6 @@ size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 size_t segment_bytes(const Shape &p, const Plan &pl) {
     return align256(sizeof(float) * pl.slots * p.heads * p.dim_k * p.dim_v);
 }
-// Of a forward call: the segments' states, and room for the state before the first token where it lies in place: the last
-// segment writes the state after the last one while others may still read it.
-size_t forward_bytes(const Shape &p, const Plan &pl) {
-    return pl.segments > 1 ? segment_bytes(p, pl) + align256(sizeof(float) * p.batch * p.heads * p.dim_k * p.dim_v) : 0;
-}
 size_t total_rows(const Shape &p) { return p.offsets ? p.rows : p.batch * p.n; }
 size_t part_bytes(const Shape &p, int heads_x, int dim) {
     return heads_x < p.heads ? align256(sizeof(float) * total_rows(p) * p.heads * dim) : 0;
@@ -418,7 +428,10 @@ int run(const Shape &p, Args &a, const Plan &pl, char *seg_ws, hipStream_t s) {
         }
         v.state_only = false;
     }
-    return launch_kernel(a, v, p.sample_type, blocks, s);
+    if (int rc = launch_kernel(a, v, p.sample_type, blocks, s)) return rc;
+    if (!a.in_place) return DSP_GPU_OK;
+    copy_states_kernel<<<static_cast<unsigned>(runs * most), 256, 0, s>>>(a);
+    return check_launch("copy_states_kernel");
 }
 
 void set_strides(long long *to, const long long *from) {
@@ -522,7 +535,7 @@ int dsp_gpu_linear_attention_workspace(const dsp_gpu_linear_attention_shape *sha
         *bytes = backward_plan(*shape).total;
     } else {
         const Plan pl = make_plan(*shape, shape->dim_k, &shape->dim_v, 1);
-        *bytes = forward_bytes(*shape, pl);
+        *bytes = segment_bytes(*shape, pl);
     }
     return DSP_GPU_OK;
 }
@@ -556,7 +569,7 @@ int dsp_gpu_linear_attention(const void *q, const void *k, const void *v, void *
     hipStream_t s = static_cast<hipStream_t>(stream);
     const Plan pl = make_plan(p, p.dim_k, &p.dim_v, 1);
     char *ws = nullptr;
-    if (int rc = take_workspace(who, rows ? forward_bytes(p, pl) : 0, workspace, workspace_bytes, s, &ws)) return rc;
+    if (int rc = take_workspace(who, rows ? segment_bytes(p, pl) : 0, workspace, workspace_bytes, s, &ws)) return rc;
     a.roles = 1;
     Role &r = a.role[0];
     fill_role(r, p, {q, p.q_stride, p.heads_q, p.dim_k}, {k, p.k_stride, p.heads_k, p.dim_k}, {v, p.v_stride, p.heads_v, p.dim_v}, o, p.o_stride, false);
@@ -566,14 +579,7 @@ int dsp_gpu_linear_attention(const void *q, const void *k, const void *v, void *
     r.s_in_d = p.dim_v;
     r.s_in_n = 1;
     r.s_out = state_out;
-    if (pl.segments > 1 && state_in && state_in == state_out) {
-        float *const before = reinterpret_cast<float *>(ws + segment_bytes(p, pl));
-        const size_t count = sb / sizeof(float), blocks = (count + 255) / 256;
-        if (blocks > 0x7fffffffu) return fail(DSP_GPU_EINVAL, "%s: %zu elements of state", who, count);
-        copy_state_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(state_in, before, count);
-        if (int rc = check_launch("copy_state_kernel")) return rc;
-        r.s_in = before;
-    }
+    a.in_place = pl.segments > 1 && state_in && state_in == state_out;
     if (int rc = run(p, a, pl, ws, s)) return rc;
     if (!p.zero_rest || !(p.offsets || p.lengths) || !rows) return DSP_GPU_OK;
     Rest z{};

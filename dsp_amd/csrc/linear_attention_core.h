@@ -72,6 +72,7 @@ struct Args {
     int heads, batch;
     int segments;                  // of the longest sequence that there can be
     unsigned slots;                // states between the segments, for each head
+    int in_place;                  // s_out is s_in, and there are segments (copy_states_kernel)
     long long seg_len;             // tokens of a segment, a multiple of the chunk
     long long n;                   // tokens of a sequence at most
     long long rows;                // rows of a packed batch
@@ -649,7 +650,7 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
 
     float *s_out = nullptr;
     if constexpr (STATE_ONLY) s_out = seg(segment);
-    else if (role.s_out && u1 == len) s_out = role.s_out + bh * d1 * d2;
+    else if (role.s_out && u1 == len) s_out = a.in_place && segment > 0 ? seg(segment - 1) : role.s_out + bh * d1 * d2;
     if (s_out) {
         int rows = d1, cols = d2;  // hidden from the compiler, which would keep 64 comparisons of the loads above for the stores
         asm volatile("" : "+s"(rows), "+s"(cols));

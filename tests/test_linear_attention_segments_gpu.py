@@ -88,6 +88,24 @@ def test_padded_sequences_of_many_segments(ops, dev):
         check_backward(*a, ld, 0.3, s0[i:i + 1], do[i:i + 1, :m], d1[i:i + 1], [x[i:i + 1, :m] for x in grads], ds[i:i + 1])
 
 
+@pytest.mark.parametrize("n", [300, 600, 2000])
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+def test_states_in_place(ops, dev, kind, n):
+    """The state after the last token over the one before the first: dense, padded and packed, one segment and many, bit for
+    bit the call with two tensors (tests above hold that one to the recurrence)."""
+    b, h, dk, dv = 3, 2, 40, 136
+    q, k, v, _, s0, _ = make(dev, TYPES[kind], b, n, h, h, h, h, dk, dv, seed=12)
+    packed = [x.flatten(0, 1) for x in (q, k, v)]
+    calls = [((q, k, v), {}), ((q, k, v), dict(lengths=torch.tensor([n, 0, n // 2], device=dev))),
+             (packed, dict(offsets=torch.tensor([0, n // 3, n // 3, 3 * n], device=dev))),
+             (packed, dict(offsets=torch.tensor([5, 6, 200, 3 * n - 1], device=dev)))]
+    for args, more in calls:
+        end, both = torch.full_like(s0, math.nan), s0.clone()
+        out = ops.linear_attention(*args, SLOW[:h], scale=0.3, state=s0, new_state=end, **more)
+        again = ops.linear_attention(*args, SLOW[:h], scale=0.3, state=both, new_state=both, **more)
+        assert torch.equal(again, out) and torch.equal(both, end)
+
+
 def test_memory_of_many_short_packed_sequences(ops, dev):
     """1,000 sequences in 32,768 rows of 16 heads, max_length left out: 0.5 GB of tensors, and less than that of workspace."""
     rows, h, d = 32768, 16, 128
@@ -99,7 +117,7 @@ def test_memory_of_many_short_packed_sequences(ops, dev):
     grads = ops.linear_attention_backward(q, k, v, [-0.01] * h, out, offsets=offsets)
     torch.cuda.synchronize()
     new = (4 * rows * h * d) * 2
-    assert torch.cuda.max_memory_allocated() - before <= new + 1100 * h * d * d * 4
+    assert torch.cuda.max_memory_allocated() - before <= new + 2 ** 27
     want = ops.linear_attention(q, k, v, [-0.01] * h, offsets=offsets, max_length=33)
     assert torch.equal(out, want)
     del grads

@@ -21,8 +21,15 @@ def workspace(backward, batch, n, rows, heads, dk, dv, kind=capi.BF16, packed=Tr
 @pytest.mark.parametrize("backward", [0, 1])
 def test_packed_batches_ask_for_what_their_rows_can_hold(backward, heads, dk, dv, batch, rows):
     """A segment with another one behind it has 128 rows at least: rows / 128 states for each gradient, however many sequences
-    there are and whatever max_length is (left out: all rows), and room for the state before the first token."""
+    there are and whatever max_length is (left out: all rows)."""
     state = 4 * heads * dk * dv
-    most = (3 if backward else 1) * (rows // 128) * state + batch * state + 4096
+    most = (3 if backward else 1) * (rows // 128) * state + 4096
     for n in (rows, rows // 2):
         assert workspace(backward, batch, n, rows, heads, dk, dv) <= most
+
+
+@pytest.mark.parametrize("batch,n", [(1, 600), (2, 2048), (8, 2048), (4, 300), (3, 32768)])
+def test_dense_batches_ask_for_the_states_between_segments(batch, n):
+    """At most n / 128 segments, and a state between each two of them -- none for the one before the first token."""
+    heads, d = 2, 64
+    assert workspace(0, batch, n, 0, heads, d, d, packed=False) <= (n // 128 - 1) * batch * 4 * heads * d * d + 256
