@@ -319,7 +319,7 @@ struct Lds {
     static constexpr int kPad = Cfg<Tc>::kPad, kPadT = Cfg<Tc>::kPadT;
     static constexpr int kQ = D1P + kPad, kD = D1P + kPadT, kN = 64 * NT + kPadT, kP = C + kPad;
     float pw[2 * C + 4];  // w^|x| at C + x; in front, where the offsets of paired reads reach
-    float pm[2 * C + 4];  // the same, zero on the side that P leaves out
+    float pm[2 * C + 4];  // the same, below zero on the side that P leaves out (a weight may itself come to zero)
     Tc q[C * kQ];
     Tc k[C * kD];
     Tc v[C * kN];
@@ -373,7 +373,7 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
     for (int x = tid; x <= 2 * C; x += kThreads) {
         const float w = power(log2w, static_cast<float>(x < C ? C - x : x - C));
         lds.pw[x] = w;
-        if constexpr (!STATE_ONLY) lds.pm[x] = (late ? x <= C : x >= C) ? w : 0.0f;
+        if constexpr (!STATE_ONLY) lds.pm[x] = (late ? x <= C : x >= C) ? w : -1.0f;
     }
 
     // the state: lane holds rows 16 dt + 4g + r, column n0 + 16 (NT wave + nt) + m
@@ -521,7 +521,7 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float w = lds.pm[C + 16 * (it - jt) + m - 4 * g - r];
-                    p[x][r] = w != 0.0f ? p[x][r] * (w * pscale) : 0.0f;  // what is left out may be anything, NaN too
+                    p[x][r] = w >= 0.0f ? p[x][r] * (w * pscale) : 0.0f;  // what is left out may be anything, NaN too
                 }
                 to_lds4(lds.p + (16 * it + m) * L::kP + 16 * jt + 4 * g, p[x]);
             }
