@@ -321,8 +321,10 @@ int dsp_gpu_rotary(const void *x, void *y, int sample_type, size_t batch, size_t
  *   state_out  the state after the last one (of an empty sequence: the one before), or NULL; may be state_in
  * Forms a chunk of tokens at a time on the matrix cores, the state in fp32 registers; few long sequences are cut in time
  * and joined.  bf16: products of bf16 operands (the weighted q k products and the state as read are rounded to bf16; what
- * the state adds up is not); F16 and F32 multiply in fp32.  What is not finite reaches the outputs that the
- * formulas carry it to, and no others (no earlier token).  Outputs do not depend on anything but the inputs and the shape: repeated calls agree
+ * the state adds up is not); F16 and F32 multiply in fp32.  The products q . k of a token with an earlier one and what the
+ * state adds up have to stay below 3.4e38; nothing is held larger than the formulas have it.  What is not finite reaches
+ * the outputs that the formulas carry it to (where an infinity may have become a NaN), and no others (no earlier token).
+ * Outputs do not depend on anything but the inputs and the shape: repeated calls agree
  * bit for bit.  The memory ranges (first to last element) of what is written must not meet those of anything else.
  * workspace: dsp_gpu_linear_attention_workspace bytes, 16-byte aligned, used until the call's work is done; NULL: the
  * library's own per (device, stream), which grows -- not under capture, and not for two graphs that run at once.
