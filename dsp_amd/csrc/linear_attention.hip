@@ -156,7 +156,7 @@ struct StepArgs {
     float *state;                          // [slots][heads][d1][d2]
     const long long *slots;                // or null: row b has state b
     long long n_slots;
-    float decay_hi[kMaxHeads], decay_lo[kMaxHeads];  // the decay to 48 bits: rounded to 24 it would drift over long answers
+    float decay_hi[kMaxHeads], decay_lo[kMaxHeads];  // the decay in two parts: rounded to 24 bits it would drift over long answers
 };
 
 constexpr int kStepCols = 64;
@@ -709,9 +709,9 @@ int dsp_gpu_linear_attention_step(const void *q, const void *k, const void *v, v
     StepArgs a{};
     if (int rc = check_decay(who, log_decay, p.heads, scale, a.decay_hi)) return rc;
     for (int h = 0; h < p.heads; ++h) {
-        const double w = std::exp(log_decay[h]);
-        a.decay_hi[h] = static_cast<float>(w);
-        a.decay_lo[h] = static_cast<float>(w - a.decay_hi[h]);
+        const Decay w = two_parts(std::exp(log_decay[h]));
+        a.decay_hi[h] = w.hi;
+        a.decay_lo[h] = w.lo;
     }
     if (p.n != 1 || p.offsets || p.lengths) return fail(DSP_GPU_EINVAL, "%s: one token a row (n = 1), no offsets or lengths", who);
     if (p.batch == 0) return DSP_GPU_OK;

@@ -127,15 +127,21 @@ __device__ __forceinline__ Slots slots_of(const Args &a, int late, int b, long l
 // w^n for n >= 0, from log2 w (-inf for w = 0: w^0 is still 1)
 __device__ __forceinline__ float power(float log2w, float n) { return n == 0.0f ? 1.0f : __builtin_amdgcn_exp2f(log2w * n); }
 
-// w^n to 48 bits, for what multiplies a state again and again: rounded to 24 bits, w^C of a slow decay would be off by
-// 2^-25 every C tokens, and the state by that times the number of chunks it remembers
+// w^n as a sum of two floats, for what multiplies a state again and again: rounded to 24 bits, w^C of a slow decay would be
+// off by 2^-25 every C tokens, and the state by that times the number of chunks it remembers.  (log2 w itself has 24 bits,
+// like the weights within a chunk: the rate of the decay is off by 2^-25 of itself, over any number of tokens.)  Both parts
+// are positive, so that an infinite state times each of them is no NaN; the least lo adds nothing to a finite product.
 struct Decay {
     float hi, lo;
 };
+__host__ __device__ inline Decay two_parts(double w) {
+    float hi = static_cast<float>(w);
+    if (hi > w) hi = __builtin_bit_cast(float, __builtin_bit_cast(int, hi) - 1);
+    const float lo = static_cast<float>(w - hi), least = hi * 0x1p-40f;
+    return {hi, lo > least ? lo : least};
+}
 __device__ __forceinline__ Decay decay_over(float log2w, long long n) {
-    const double w = n == 0 ? 1.0 : exp2(static_cast<double>(log2w) * static_cast<double>(n));
-    const float hi = static_cast<float>(w);
-    return {hi, static_cast<float>(w - hi)};
+    return two_parts(n == 0 ? 1.0 : exp2(static_cast<double>(log2w) * static_cast<double>(n)));
 }
 
 template <typename Tc>

@@ -86,3 +86,26 @@ def test_large_values_and_small_ones(ops, dev, kind, log_decay):
         factor = [max(mq, mv), mk, max(mk, mdo), max(mq, mv), max(mk, mdo), mq]
         for i, (x, w, t, f) in enumerate(zip((out, end, *grads, ds), want, total, factor)):
             near(x, w, t, terms, x.dtype, f, operands=i not in (1, 5))
+
+
+@pytest.mark.parametrize("n", [1, 64, 150, 700, 1400])
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+def test_an_infinite_state_stays_infinite(ops, dev, kind, n):
+    """w * inf = inf for every decay but zero, whichever way w^n rounds: after single tokens, a few chunks, and segments."""
+    b, h, dk, dv = 1, 12, 24, 40
+    q, k, v, _, s0, _ = make(dev, TYPES[kind], b, n, h, h, h, h, dk, dv, seed=14)
+    ld = [0.0, -0.001, -0.002, -0.003, -0.01, -0.011, -0.02, -0.03, math.log(0.5) / 64, -0.1, -0.2, -0.3]
+    s0[:, :, 3, 5], s0[:, :, 7, 6] = math.inf, -math.inf
+    args = [x.cpu().double() for x in (q, k, v)]
+    want, wend = ref.forward(*args, ld, 0.3, s0)
+    end = torch.empty_like(s0)
+    out = ops.linear_attention(q, k, v, ld, scale=0.3, state=s0, new_state=end)
+    odd = ~torch.isfinite(wend)
+    assert odd.sum() == 2 * h and torch.equal(end.cpu()[odd].double(), wend[odd]) and torch.isfinite(end.cpu()[~odd]).all()
+    assert torch.equal(torch.isfinite(out.cpu()), torch.isfinite(want))
+    if n == 1:
+        state = s0.clone()
+        one = ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state, scale=0.3)
+        odd_o = ~torch.isfinite(want[:, 0])
+        assert torch.equal(state.cpu()[odd].double(), wend[odd]) and torch.isfinite(state.cpu()[~odd]).all()
+        assert torch.equal(one.cpu()[odd_o].double(), want[:, 0][odd_o]) and torch.isfinite(one.cpu()[~odd_o]).all()
