@@ -17,10 +17,11 @@ namespace {
 // A thread has kJoin elements of the state, 256 apart; the loads do not depend on the recurrence.
 constexpr int kJoin = 4;
 __global__ void __launch_bounds__(256) join_segments_kernel(const Args a) {
-    const Role &role = a.role[blockIdx.y];
+    const Role &role = a.role[blockIdx.z];
     const int count = role.d1 * role.d2, blocks = (count + 256 * kJoin - 1) / (256 * kJoin);
-    const int bh = blockIdx.x / blocks, e0 = (blockIdx.x % blocks) * 256 * kJoin + threadIdx.x;
-    if (bh >= a.batch * a.heads) return;
+    const unsigned id = static_cast<unsigned>(block_index());
+    if (id / blocks >= static_cast<unsigned>(a.batch * a.heads)) return;
+    const int bh = id / blocks, e0 = (id % blocks) * 256 * kJoin + threadIdx.x;
     long long start, len;
     sequence_rows(a, bh / a.heads, start, len);
     const int full = inner_segments(a, len);
@@ -59,8 +60,9 @@ __global__ void __launch_bounds__(256) join_segments_kernel(const Args a) {
 __global__ void __launch_bounds__(256) copy_states_kernel(const Args a) {
     const Role &role = a.role[0];
     const int count = role.d1 * role.d2, blocks = (count + 256 * kJoin - 1) / (256 * kJoin);
-    const int bh = blockIdx.x / blocks, e0 = (blockIdx.x % blocks) * 256 * kJoin + threadIdx.x;
-    if (bh >= a.batch * a.heads) return;
+    const unsigned id = static_cast<unsigned>(block_index());
+    if (id / blocks >= static_cast<unsigned>(a.batch * a.heads)) return;
+    const int bh = id / blocks, e0 = (id % blocks) * 256 * kJoin + threadIdx.x;
     long long start, len;
     sequence_rows(a, bh / a.heads, start, len);
     const int full = inner_segments(a, len);
@@ -91,14 +93,15 @@ struct Shared {
     const float *part[3];
     void *out[3];
     int group[3], dim[3];
+    long long rows;
 };
 
 // part [row][heads][dim] fp32 -> out [row][heads / group][dim], heads of a group added in their order
 template <typename T>
 __global__ void __launch_bounds__(256) add_heads_kernel(const Args a, const Shared g) {
-    const long long row = blockIdx.x;
-    if (!row_taken(a, row)) return;
-    const int i = blockIdx.y, group = g.group[i], dim = g.dim[i], heads = a.heads / group;
+    const long long row = static_cast<long long>(block_index());
+    if (row >= g.rows || !row_taken(a, row)) return;
+    const int i = blockIdx.z, group = g.group[i], dim = g.dim[i], heads = a.heads / group;
     for (int e = threadIdx.x; e < heads * dim; e += 256) {
         const float *p = g.part[i] + (row * a.heads + (e / dim) * group) * dim + e % dim;
         float sum = 0.0f;
@@ -123,10 +126,10 @@ __global__ void __launch_bounds__(256) zero_rest_kernel(const Args a, const Rest
     __shared__ int list[256], count;
     if (threadIdx.x == 0) count = 0;
     __syncthreads();
-    const long long first = static_cast<long long>(blockIdx.x) * 256, mine = first + threadIdx.x;
+    const long long first = static_cast<long long>(block_index()) * 256, mine = first + threadIdx.x;
     if (mine < z.rows && !row_taken(a, mine)) list[atomicAdd(&count, 1)] = threadIdx.x;
     __syncthreads();
-    const int i = blockIdx.y;
+    const int i = blockIdx.z;
     for (int r = 0; r < count; ++r) {
         const long long row = first + list[r];
         const long long at = a.offsets ? row * z.stride[i][1] : row / a.n * z.stride[i][0] + row % a.n * z.stride[i][1];
@@ -139,7 +142,7 @@ __global__ void __launch_bounds__(256) zero_rest_kernel(const Args a, const Rest
 }
 
 int zero_rest(const Args &a, Rest &z, int count, hipStream_t s) {
-    zero_rest_kernel<<<dim3(static_cast<unsigned>((z.rows + 255) / 256), count), 256, 0, s>>>(a, z);
+    zero_rest_kernel<<<grid_of(static_cast<size_t>((z.rows + 255) / 256), count), 256, 0, s>>>(a, z);
     return check_launch("zero_rest_kernel");
 }
 
@@ -170,8 +173,10 @@ __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
     __shared__ float part[4][kStepCols];
     __shared__ int first, more;
     const int tiles = (a.d2 + kStepCols - 1) / kStepCols;
-    const int tile = blockIdx.x % tiles, head = blockIdx.x / tiles % a.heads;
-    int b = blockIdx.x / tiles / a.heads;
+    const unsigned id = static_cast<unsigned>(block_index());
+    const int tile = id % tiles, head = id / tiles % a.heads;
+    int b = id / tiles / a.heads;
+    if (b >= a.batch) return;
     const int tid = threadIdx.x, cx = tid & 15, ry = tid >> 4, lane = tid & 63, wave = tid >> 6;
     const int n0 = tile * kStepCols + 4 * cx;
 
@@ -275,10 +280,10 @@ __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
 
 template <typename T>
 int launch_step(const StepArgs &a, hipStream_t s) {
-    const unsigned blocks = static_cast<unsigned>(static_cast<size_t>(a.batch) * a.heads * ((a.d2 + kStepCols - 1) / kStepCols));
-    if (a.d1 <= 64) step_kernel<T, 4><<<blocks, 256, 0, s>>>(a);
-    else if (a.d1 <= 128) step_kernel<T, 8><<<blocks, 256, 0, s>>>(a);
-    else step_kernel<T, 16><<<blocks, 256, 0, s>>>(a);
+    const dim3 grid = grid_of(static_cast<size_t>(a.batch) * a.heads * ((a.d2 + kStepCols - 1) / kStepCols));
+    if (a.d1 <= 64) step_kernel<T, 4><<<grid, 256, 0, s>>>(a);
+    else if (a.d1 <= 128) step_kernel<T, 8><<<grid, 256, 0, s>>>(a);
+    else step_kernel<T, 16><<<grid, 256, 0, s>>>(a);
     return check_launch("step_kernel");
 }
 
@@ -388,11 +393,11 @@ size_t part_bytes(const Shape &p, int heads_x, int dim) {
     return heads_x < p.heads ? align256(sizeof(float) * total_rows(p) * p.heads * dim) : 0;
 }
 
-int launch_kernel(const Args &a, const Variant &v, int type, size_t blocks, hipStream_t s) {
-    const unsigned n = static_cast<unsigned>(blocks);
-    if (type == DSP_GPU_BF16) return launch_bf16(a, v, n, s);
-    if (type == DSP_GPU_F16) return launch_f16(a, v, n, s);
-    return launch_f32(a, v, n, s);
+int launch_kernel(Args &a, const Variant &v, int type, size_t blocks, hipStream_t s) {
+    a.blocks = static_cast<unsigned>(blocks);
+    if (type == DSP_GPU_BF16) return launch_bf16(a, v, s);
+    if (type == DSP_GPU_F16) return launch_f16(a, v, s);
+    return launch_f32(a, v, s);
 }
 
 // roles: a.role[0 .. a.roles) with everything but tiles and seg filled in; seg_ws: a.roles * segment_bytes
@@ -423,14 +428,14 @@ int run(const Shape &p, Args &a, const Plan &pl, char *seg_ws, hipStream_t s) {
         v.state_only = true;
         if (int rc = launch_kernel(a, v, p.sample_type, inner, s)) return rc;
         if (pl.segments > kJoinSelf) {
-            join_segments_kernel<<<dim3(static_cast<unsigned>(runs * most), a.roles), 256, 0, s>>>(a);
+            join_segments_kernel<<<grid_of(runs * most, a.roles), 256, 0, s>>>(a);
             if (int rc = check_launch("join_segments_kernel")) return rc;
         }
         v.state_only = false;
     }
     if (int rc = launch_kernel(a, v, p.sample_type, blocks, s)) return rc;
     if (!a.in_place) return DSP_GPU_OK;
-    copy_states_kernel<<<static_cast<unsigned>(runs * most), 256, 0, s>>>(a);
+    copy_states_kernel<<<grid_of(runs * most), 256, 0, s>>>(a);
     return check_launch("copy_states_kernel");
 }
 
@@ -510,7 +515,7 @@ int take_workspace(const char *who, size_t need, void *given, size_t given_bytes
 
 template <typename T>
 int add_heads(const Args &a, const Shape &p, const Shared &g, int count, hipStream_t s) {
-    add_heads_kernel<T><<<dim3(static_cast<unsigned>(total_rows(p)), count), 256, 0, s>>>(a, g);
+    add_heads_kernel<T><<<grid_of(total_rows(p), count), 256, 0, s>>>(a, g);
     return check_launch("add_heads_kernel");
 }
 
@@ -670,6 +675,7 @@ int dsp_gpu_linear_attention_backward(const void *q, const void *k, const void *
         if (int rc = run(p, a, bp.pl[2], ws, s)) return rc;
     }
     Shared g{};
+    g.rows = static_cast<long long>(rows);
     int count = 0;
     for (int i = 0; i < 3; ++i) {
         if (!part[i] || !rows) continue;

@@ -4,8 +4,8 @@
 namespace dspgpu {
 namespace la {
 
-int launch_bf16(const Args &a, const Variant &v, unsigned blocks, hipStream_t s) {
-    return launch_any<__bf16, __bf16>(a, v, blocks, s);
+int launch_bf16(const Args &a, const Variant &v, hipStream_t s) {
+    return launch_any<__bf16, __bf16>(a, v, s);
 }
 
 }  // namespace la

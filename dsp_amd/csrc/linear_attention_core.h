@@ -70,6 +70,7 @@ struct Args {
     Role role[kMaxRoles];
     int roles;
     int heads, batch;
+    unsigned blocks;               // workgroups that have work
     int segments;                  // of the longest sequence that there can be
     unsigned slots;                // states between the segments, for each head
     int in_place;                  // s_out is s_in, and there are segments (copy_states_kernel)
@@ -670,7 +671,8 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
 template <typename Ti, typename Tc, int D1P, int NT, int C, bool STATE_ONLY, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Args a) {
     // workgroup -> (segment of a sequence, head, role, tile): the tiles and roles of a head next to each other
-    unsigned id = blockIdx.x;
+    unsigned id = static_cast<unsigned>(block_index());
+    if (id >= a.blocks) return;
     unsigned role_tiles = 0;
     for (int r = 0; r < a.roles; ++r) role_tiles += a.role[r].tiles;
     int t = id % role_tiles;
@@ -710,13 +712,13 @@ __global__ void __launch_bounds__(kThreads, 2) linear_attention_kernel(const Arg
 
 // D1P and NT by the host's rule; C by the type: 64 tokens, 32 where an element is four bytes or a row 256 of them (LDS)
 template <typename Ti, typename Tc, int D1P, int NT, bool STATE_ONLY, bool VEC>
-int launch_kernel_as(const Args &a, unsigned blocks, hipStream_t s) {
+int launch_kernel_as(const Args &a, hipStream_t s) {
     constexpr int C = sizeof(Tc) == 2 && D1P <= 128 ? 64 : 32;
     using L = typename std::conditional<STATE_ONLY, LdsState<Tc, D1P, NT, C>, Lds<Tc, D1P, NT, C>>::type;
     const auto fn = linear_attention_kernel<Ti, Tc, D1P, NT, C, STATE_ONLY, VEC>;
     if (sizeof(L) > 65536)
         if (int rc = allow_full_lds(reinterpret_cast<const void *>(fn))) return rc;
-    fn<<<blocks, kThreads, sizeof(L), s>>>(a);
+    fn<<<grid_of(a.blocks), kThreads, sizeof(L), s>>>(a);
     return check_launch("linear_attention_kernel");
 }
 
@@ -726,22 +728,22 @@ struct Variant {
 };
 
 template <typename Ti, typename Tc, int D1P, int NT>
-int launch_one(const Args &a, const Variant &v, unsigned blocks, hipStream_t s) {
-    if (v.state_only) return v.vec ? launch_kernel_as<Ti, Tc, D1P, NT, true, true>(a, blocks, s) : launch_kernel_as<Ti, Tc, D1P, NT, true, false>(a, blocks, s);
-    return v.vec ? launch_kernel_as<Ti, Tc, D1P, NT, false, true>(a, blocks, s) : launch_kernel_as<Ti, Tc, D1P, NT, false, false>(a, blocks, s);
+int launch_one(const Args &a, const Variant &v, hipStream_t s) {
+    if (v.state_only) return v.vec ? launch_kernel_as<Ti, Tc, D1P, NT, true, true>(a, s) : launch_kernel_as<Ti, Tc, D1P, NT, true, false>(a, s);
+    return v.vec ? launch_kernel_as<Ti, Tc, D1P, NT, false, true>(a, s) : launch_kernel_as<Ti, Tc, D1P, NT, false, false>(a, s);
 }
 
 template <typename Ti, typename Tc>
-int launch_any(const Args &a, const Variant &v, unsigned blocks, hipStream_t s) {
-    if (v.d1p == 64) return v.nt == 1 ? launch_one<Ti, Tc, 64, 1>(a, v, blocks, s) : launch_one<Ti, Tc, 64, 2>(a, v, blocks, s);
-    if (v.d1p == 128) return v.nt == 1 ? launch_one<Ti, Tc, 128, 1>(a, v, blocks, s) : launch_one<Ti, Tc, 128, 2>(a, v, blocks, s);
-    return launch_one<Ti, Tc, 256, 1>(a, v, blocks, s);
+int launch_any(const Args &a, const Variant &v, hipStream_t s) {
+    if (v.d1p == 64) return v.nt == 1 ? launch_one<Ti, Tc, 64, 1>(a, v, s) : launch_one<Ti, Tc, 64, 2>(a, v, s);
+    if (v.d1p == 128) return v.nt == 1 ? launch_one<Ti, Tc, 128, 1>(a, v, s) : launch_one<Ti, Tc, 128, 2>(a, v, s);
+    return launch_one<Ti, Tc, 256, 1>(a, v, s);
 }
 
 // one translation unit each
-int launch_bf16(const Args &a, const Variant &v, unsigned blocks, hipStream_t s);
-int launch_f16(const Args &a, const Variant &v, unsigned blocks, hipStream_t s);
-int launch_f32(const Args &a, const Variant &v, unsigned blocks, hipStream_t s);
+int launch_bf16(const Args &a, const Variant &v, hipStream_t s);
+int launch_f16(const Args &a, const Variant &v, hipStream_t s);
+int launch_f32(const Args &a, const Variant &v, hipStream_t s);
 
 }  // namespace la
 }  // namespace dspgpu

@@ -4,8 +4,8 @@
 namespace dspgpu {
 namespace la {
 
-int launch_f16(const Args &a, const Variant &v, unsigned blocks, hipStream_t s) {
-    return launch_any<_Float16, float>(a, v, blocks, s);
+int launch_f16(const Args &a, const Variant &v, hipStream_t s) {
+    return launch_any<_Float16, float>(a, v, s);
 }
 
 }  // namespace la

@@ -4,8 +4,8 @@
 namespace dspgpu {
 namespace la {
 
-int launch_f32(const Args &a, const Variant &v, unsigned blocks, hipStream_t s) {
-    return launch_any<float, float>(a, v, blocks, s);
+int launch_f32(const Args &a, const Variant &v, hipStream_t s) {
+    return launch_any<float, float>(a, v, s);
 }
 
 }  // namespace la

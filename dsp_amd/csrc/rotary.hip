@@ -39,7 +39,7 @@ struct alignas(sizeof(T) * VE) Vec {
 // VE elements a load; HALF: VE pairs a thread (two loads), else VE / 2 pairs (one load).  WIDE: rows are aligned to a load.
 template <typename T, int VE, bool HALF, bool WIDE>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
-    const unsigned long long id = static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x;
+    const unsigned long long id = static_cast<unsigned long long>(block_index()) * 256 + threadIdx.x;
     if (id >= a.threads) return;
     unsigned long long token;
     int chunk, lane;
@@ -133,8 +133,8 @@ int launch(RotaryArgs &a, size_t rows, bool copy, hipStream_t s) {
     a.head_lanes = (a.heads + reuse - 1) / reuse;
     a.threads = static_cast<unsigned long long>(rows) * a.chunks * a.head_lanes;
     const unsigned long long blocks = (a.threads + 255) / 256;
-    if (blocks > 0x7fffffffu) return fail(DSP_GPU_EINVAL, "dsp_gpu_rotary: %llu workgroups", blocks);
-    rotary_kernel<T, VE, HALF, WIDE><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+    if (blocks > kMostBlocks) return fail(DSP_GPU_EINVAL, "dsp_gpu_rotary: %llu workgroups", blocks);
+    rotary_kernel<T, VE, HALF, WIDE><<<grid_of(blocks), 256, 0, s>>>(a);
     return check_launch("rotary_kernel");
 }
 
