@@ -54,6 +54,8 @@ inline bool rows_distinct(const long long *stride, size_t batch, size_t n, size_
     return true;
 }
 
+// ---- streaming helpers shared by the kernels (device side) ------------------------------------
+#if defined(__HIPCC__)
 // An axis of a launch holds fewer than 2^32 threads (more of them wrap, with no error): `blocks` workgroups of up to 1,024
 // threads over x and y, at most a row of x too many.  The kernel takes block_index() and leaves out what is not below `blocks`.
 constexpr size_t kGridRow = size_t(1) << 21;
@@ -62,9 +64,6 @@ inline dim3 grid_of(size_t blocks, unsigned z = 1) {
     return dim3(static_cast<unsigned>(kGridRow), static_cast<unsigned>((blocks + kGridRow - 1) / kGridRow), z);
 }
 constexpr size_t kMostBlocks = kGridRow * 65535;
-
-// ---- streaming helpers shared by the kernels (device side) ------------------------------------
-#if defined(__HIPCC__)
 __device__ __forceinline__ size_t block_index() { return static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
 
 typedef float dsp_f32x4 __attribute__((ext_vector_type(4)));
