@@ -54,6 +54,15 @@ inline bool rows_distinct(const long long *stride, size_t batch, size_t n, size_
     return true;
 }
 
+// Whether a strided [batch][n][heads][dim] array ends within 2^44 elements: no memory is larger, and no sum of steps wraps.
+inline bool extent_fits(const long long *stride, size_t batch, size_t n, size_t heads, size_t dim) {
+    unsigned __int128 e = dim;
+    if (batch > 1) e += static_cast<unsigned __int128>(batch - 1) * static_cast<size_t>(stride[0]);
+    if (n > 1) e += static_cast<unsigned __int128>(n - 1) * static_cast<size_t>(stride[1]);
+    if (heads > 1) e += static_cast<unsigned __int128>(heads - 1) * static_cast<size_t>(stride[2]);
+    return e <= (static_cast<unsigned __int128>(1) << 44);
+}
+
 // ---- streaming helpers shared by the kernels (device side) ------------------------------------
 #if defined(__HIPCC__)
 // An axis of a launch holds fewer than 2^32 threads (more of them wrap, with no error): `blocks` workgroups of up to 1,024

@@ -301,6 +301,7 @@ bool meet(const Range &a, const Range &b) { return a.p && b.p && a.bytes && b.by
 
 // bytes from the first to the last element of a strided [batch][n][heads][dim] array
 size_t extent(const long long *stride, size_t batch, size_t n, size_t heads, size_t dim, size_t size) {
+    if (batch == 0 || n == 0) return 0;
     return ((batch - 1) * stride[0] + (n - 1) * stride[1] + (heads - 1) * stride[2] + dim) * size;
 }
 
@@ -330,7 +331,35 @@ int check_shape(const char *who, const Shape &p) {
     for (const long long *s : {p.q_stride, p.k_stride, p.v_stride, p.o_stride})
         for (int i = 0; i < 3; ++i)
             if (s[i] < 0 || s[i] > (1ll << 40)) return fail(DSP_GPU_EINVAL, "%s: stride %lld", who, s[i]);
+    const size_t batch = p.offsets ? 1 : p.batch, n = p.offsets ? p.rows : p.n;
+    if (!extent_fits(p.q_stride, batch, n, p.heads_q, p.dim_k) || !extent_fits(p.k_stride, batch, n, p.heads_k, p.dim_k) ||
+        !extent_fits(p.v_stride, batch, n, p.heads_v, p.dim_v) || !extent_fits(p.o_stride, batch, n, p.heads, p.dim_v))
+        return fail(DSP_GPU_EINVAL, "%s: a tensor is larger than any memory", who);
     return DSP_GPU_OK;
+}
+
+// Ranges that a call reads or writes: what it writes must not meet any other.  Empty and null ranges meet nothing.
+struct Buffers {
+    Range r[12];
+    int count = 0;
+    void add(const void *p, size_t bytes) { r[count++] = {static_cast<const char *>(p), bytes}; }
+    bool meet(const void *p, size_t bytes) const {
+        for (int i = 0; i < count; ++i)
+            if (la::meet({static_cast<const char *>(p), bytes}, r[i])) return true;
+        return false;
+    }
+};
+
+// the inputs that forward and backward share
+Buffers inputs(const Shape &p, const void *q, const void *k, const void *v) {
+    const size_t batch = p.offsets ? 1 : p.batch, n = p.offsets ? p.rows : p.n, size = sample_bytes(p.sample_type);
+    Buffers b;
+    b.add(q, extent(p.q_stride, batch, n, p.heads_q, p.dim_k, size));
+    b.add(k, extent(p.k_stride, batch, n, p.heads_k, p.dim_k, size));
+    b.add(v, extent(p.v_stride, batch, n, p.heads_v, p.dim_v, size));
+    b.add(p.offsets, sizeof(long long) * (p.batch + 1));
+    b.add(p.lengths, sizeof(long long) * p.batch);
+    return b;
 }
 
 // One launch of the kernel: up to three roles that share the padded first dimension and the columns of a workgroup.
@@ -498,12 +527,13 @@ BackwardPlan backward_plan(const Shape &p) {
     return bp;
 }
 
-int take_workspace(const char *who, size_t need, void *given, size_t given_bytes, hipStream_t s, char **out) {
+int take_workspace(const char *who, size_t need, void *given, size_t given_bytes, const Buffers &used, hipStream_t s, char **out) {
     *out = nullptr;
     if (need == 0) return DSP_GPU_OK;
     if (given) {
         if (given_bytes < need) return fail(DSP_GPU_EINVAL, "%s: a workspace of %zu bytes, %zu are needed", who, given_bytes, need);
         if (reinterpret_cast<uintptr_t>(given) % 16) return fail(DSP_GPU_EINVAL, "%s: workspace not aligned to 16 bytes", who);
+        if (used.meet(given, need)) return fail(DSP_GPU_EINVAL, "%s: the workspace overlaps a buffer", who);
         *out = static_cast<char *>(given);
         return DSP_GPU_OK;
     }
@@ -558,23 +588,18 @@ int dsp_gpu_linear_attention(const void *q, const void *k, const void *v, void *
     if (p.batch == 0 && !(p.zero_rest && rows)) return DSP_GPU_OK;
     if (rows && (!q || !k || !v || !o)) return fail(DSP_GPU_EINVAL, "%s: null buffer", who);
     const size_t size = sample_bytes(p.sample_type), sb = state_bytes(p);
-    if (rows) {
-        const size_t batch = p.offsets ? 1 : p.batch, n = p.offsets ? p.rows : p.n;
-        if (!rows_distinct(p.o_stride, batch, n, p.heads, p.dim_v)) return fail(DSP_GPU_EINVAL, "%s: rows of o overlap one another", who);
-        const Range ro{static_cast<const char *>(o), extent(p.o_stride, batch, n, p.heads, p.dim_v, size)};
-        const Range rs_in{reinterpret_cast<const char *>(state_in), sb}, rs_out{reinterpret_cast<const char *>(state_out), sb};
-        for (const Range &x : {Range{static_cast<const char *>(q), extent(p.q_stride, batch, n, p.heads_q, p.dim_k, size)},
-                               Range{static_cast<const char *>(k), extent(p.k_stride, batch, n, p.heads_k, p.dim_k, size)},
-                               Range{static_cast<const char *>(v), extent(p.v_stride, batch, n, p.heads_v, p.dim_v, size)}})
-            if (meet(x, ro) || meet(x, rs_out)) return fail(DSP_GPU_EINVAL, "%s: an output overlaps q, k or v", who);
-        if (meet(ro, rs_in) || meet(ro, rs_out)) return fail(DSP_GPU_EINVAL, "%s: o overlaps a state", who);
-    }
-    if (state_in != state_out && meet({reinterpret_cast<const char *>(state_in), sb}, {reinterpret_cast<const char *>(state_out), sb}))
-        return fail(DSP_GPU_EINVAL, "%s: the states overlap", who);
+    const size_t batch = p.offsets ? 1 : p.batch, n = p.offsets ? p.rows : p.n, ob = extent(p.o_stride, batch, n, p.heads, p.dim_v, size);
+    if (rows && !rows_distinct(p.o_stride, batch, n, p.heads, p.dim_v)) return fail(DSP_GPU_EINVAL, "%s: rows of o overlap one another", who);
+    Buffers used = inputs(p, q, k, v);
+    if (state_in != state_out) used.add(state_in, sb);
+    if (used.meet(o, ob)) return fail(DSP_GPU_EINVAL, "%s: o overlaps an input", who);
+    used.add(o, ob);
+    if (used.meet(state_out, sb)) return fail(DSP_GPU_EINVAL, "%s: state_out overlaps something else", who);
+    used.add(state_out, sb);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const Plan pl = make_plan(p, p.dim_k, &p.dim_v, 1);
     char *ws = nullptr;
-    if (int rc = take_workspace(who, rows ? segment_bytes(p, pl) : 0, workspace, workspace_bytes, s, &ws)) return rc;
+    if (int rc = take_workspace(who, rows ? segment_bytes(p, pl) : 0, workspace, workspace_bytes, used, s, &ws)) return rc;
     a.roles = 1;
     Role &r = a.role[0];
     fill_role(r, p, {q, p.q_stride, p.heads_q, p.dim_k}, {k, p.k_stride, p.heads_k, p.dim_k}, {v, p.v_stride, p.heads_v, p.dim_v}, o, p.o_stride, false);
@@ -611,31 +636,23 @@ int dsp_gpu_linear_attention_backward(const void *q, const void *k, const void *
     if (p.batch == 0 && !(p.zero_rest && rows)) return DSP_GPU_OK;
     if (rows && (!q || !k || !v || !dout || !dq || !dk || !dv)) return fail(DSP_GPU_EINVAL, "%s: null buffer", who);
     if (rows > 0x7fffffffu) return fail(DSP_GPU_EINVAL, "%s: %zu rows", who, rows);
-    if (rows) {
-        const size_t batch = p.offsets ? 1 : p.batch, n = p.offsets ? p.rows : p.n;
-        const Range out[4] = {{static_cast<const char *>(dq), rows * p.heads_q * p.dim_k * size},
-                              {static_cast<const char *>(dk), rows * p.heads_k * p.dim_k * size},
-                              {static_cast<const char *>(dv), rows * p.heads_v * p.dim_v * size},
-                              {reinterpret_cast<const char *>(dstate_in), sb}};
-        const Range in[5] = {{static_cast<const char *>(q), extent(p.q_stride, batch, n, p.heads_q, p.dim_k, size)},
-                             {static_cast<const char *>(k), extent(p.k_stride, batch, n, p.heads_k, p.dim_k, size)},
-                             {static_cast<const char *>(v), extent(p.v_stride, batch, n, p.heads_v, p.dim_v, size)},
-                             {static_cast<const char *>(dout), extent(p.o_stride, batch, n, p.heads, p.dim_v, size)},
-                             {reinterpret_cast<const char *>(state_in), sb}};
-        for (int i = 0; i < 4; ++i) {
-            for (const Range &x : in)
-                if (meet(out[i], x)) return fail(DSP_GPU_EINVAL, "%s: a gradient overlaps an input", who);
-            for (int j = 0; j < i; ++j)
-                if (meet(out[i], out[j])) return fail(DSP_GPU_EINVAL, "%s: two gradients overlap", who);
-        }
+    const size_t batch = p.offsets ? 1 : p.batch, n = p.offsets ? p.rows : p.n;
+    Buffers used = inputs(p, q, k, v);
+    used.add(dout, extent(p.o_stride, batch, n, p.heads, p.dim_v, size));
+    used.add(state_in, sb);
+    used.add(dstate_out, sb);  // dk reads it while dv writes dstate_in: not in place
+    const struct {
+        const void *p;
+        size_t bytes;
+    } written[4] = {{dq, rows * p.heads_q * p.dim_k * size}, {dk, rows * p.heads_k * p.dim_k * size}, {dv, rows * p.heads_v * p.dim_v * size}, {dstate_in, sb}};
+    for (const auto &x : written) {
+        if (used.meet(x.p, x.bytes)) return fail(DSP_GPU_EINVAL, "%s: a gradient overlaps an input or another gradient", who);
+        used.add(x.p, x.bytes);
     }
-    // dk reads dstate_out while dv writes dstate_in: not in place
-    if (meet({reinterpret_cast<const char *>(dstate_in), sb}, {reinterpret_cast<const char *>(dstate_out), sb}))
-        return fail(DSP_GPU_EINVAL, "%s: dstate_in and dstate_out overlap", who);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const BackwardPlan bp = backward_plan(p);
     char *ws = nullptr;
-    if (int rc = take_workspace(who, rows ? bp.total : 0, workspace, workspace_bytes, s, &ws)) return rc;
+    if (int rc = take_workspace(who, rows ? bp.total : 0, workspace, workspace_bytes, used, s, &ws)) return rc;
 
     const Tensor tq{q, p.q_stride, p.heads_q, p.dim_k}, tk{k, p.k_stride, p.heads_k, p.dim_k}, tv{v, p.v_stride, p.heads_v, p.dim_v},
         tdo{dout, p.o_stride, p.heads, p.dim_v};

@@ -189,6 +189,12 @@ extern "C" int dsp_gpu_rotary(const void *x, void *y, int sample_type, size_t ba
     if (positions && (position_stride[0] < 0 || position_stride[1] < 0)) return fail(DSP_GPU_EINVAL, "%s: negative position stride", who);
     if (batch == 0 || n == 0) return DSP_GPU_OK;
     if (!x || !y) return fail(DSP_GPU_EINVAL, "%s: null buffer", who);
+    if (!extent_fits(x_stride, batch, n, heads, dim) || !extent_fits(y_stride, batch, n, heads, dim))
+        return fail(DSP_GPU_EINVAL, "%s: x or y is larger than any memory", who);
+    if (positions) {
+        const long long st[3] = {position_stride[0], position_stride[1], 0};
+        if (!extent_fits(st, batch, n, 1, 1)) return fail(DSP_GPU_EINVAL, "%s: positions are larger than any memory", who);
+    }
     if (!rows_distinct(y_stride, batch, n, heads, dim)) return fail(DSP_GPU_EINVAL, "%s: rows of y overlap one another", who);
     const size_t size = sample_type == DSP_GPU_F32 ? 4 : 2;
     auto bytes = [&](const long long *st) { return ((batch - 1) * st[0] + (n - 1) * st[1] + (heads - 1) * st[2] + dim) * size; };
