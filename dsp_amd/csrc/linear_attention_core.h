@@ -178,6 +178,16 @@ __device__ __forceinline__ void settle(f32x4 (&x)[N]) {
     if constexpr (N == 1) settle(x[0]);
 }
 
+// Two wait states between what inline assembly has written and the matrix products that read it: hipcc puts them behind vector
+// instructions that it knows of.
+template <int N>
+__device__ __forceinline__ void ready(f32x4 (&x)[N]) {
+    static_assert(N == 4 || N == 8 || N == 16, "states of 64, 128, 256 rows");
+    if constexpr (N >= 8) asm volatile("s_nop 1" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]));
+    if constexpr (N == 16) asm volatile("s_nop 1" : "+v"(x[8]), "+v"(x[9]), "+v"(x[10]), "+v"(x[11]), "+v"(x[12]), "+v"(x[13]), "+v"(x[14]), "+v"(x[15]));
+    if constexpr (N == 4) asm volatile("s_nop 1" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+}
+
 // adds 0 if all of a lane group's elements are finite, else NaN somewhere
 __device__ __forceinline__ void times_zero(f32x4 &acc, bf16x8 a) { mma(acc, a, bf16x8{}); }
 __device__ __forceinline__ void times_zero(f32x4 &acc, f32x8 a) {
@@ -614,6 +624,7 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
                 asm("v_mul_f32 %1, %2, %0\n\tv_fma_f32 %0, %0, %3, %1" : "+v"(x), "=&v"(t) : "v"(lo), "v"(hi));
                 S[i][r] = x;
             }
+        ready(S);
 #pragma unroll
         for (int jb = 0; jb < JB; ++jb) {
             float wj[8];
