@@ -166,7 +166,7 @@ constexpr int kStepCols = 64;
 
 // S <- w S + k v^T, o = scale q S.  Bound by the state's traffic (8 d1 d2 bytes a head): a workgroup takes 64 columns of one
 // head, each thread four columns of every 16th row, all its rows in flight at once, and the operands beside them.  64 rows
-// of 16 heads of 128 x 128: 27 us for 134 MB, 4.9 TB/s; one row of 8 heads of 64 x 64: 5 us, a launch and three latencies.
+// of 16 heads of 128 x 128: 28 us for 134 MB, 4.8 TB/s; one row of 8 heads of 64 x 64: 5 us, a launch and three latencies.
 // A slot that several rows name is taken by the workgroup of the first of them, for all of them in their order.
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
@@ -370,15 +370,16 @@ struct Plan {
 };
 
 constexpr long long kSlots = 512;     // workgroups the chip runs at once: two on each of 256 CUs
-// Tokens of a segment at least: a state is written and read for each.  (2 x 1000 tokens of 12 heads, backward: 65 us; 256:
-// 89 us.  1 x 600 of 4 heads: 33 us; 256: 45 us, 64: 30 us, but 8 x 2048 of 16 heads 2 % slower.)
+// Tokens of a segment at least: a state is written and read for each.  (2 x 1000 tokens of 12 heads of 48 x 80, backward:
+// 55 us; 256: 65 us, 64: 56 us.  2 x 2048 of 8 heads, fp32: 47 us; 256: 66 us, 64: 48 us.  1 x 600 of 4 heads: 34 us; 256:
+// 48 us, 64: 30 us.)
 constexpr long long kLeast = 128;
 
 // How the work of `roles` runs over batch * heads sequences is spread.  A workgroup that owns 128 columns reads q and k half
 // as often as two that own 64.  Where the runs do not fill the chip the time axis is cut into segments, which costs a
 // second pass over k and v (about kAgain of the first): dense batches take the number of segments with the least
 // ceil(workgroups / slots) * tokens of a segment; of packed ones only the sum of the lengths is known, and a segment is
-// its share of a slot (20,011 tokens of 16 heads in 16 sequences: 208 us; half of it 225 us, a third 237 us).
+// its share of a slot (20,011 tokens of 16 heads in 16 sequences: 175 us; half of it 191 us, a third 197 us).
 Plan make_plan(const Shape &p, int d1, const int *d2, int roles) {
     Plan pl{};
     pl.d1p = d1 <= 64 ? 64 : d1 <= 128 ? 128 : 256;
@@ -507,8 +508,8 @@ BackwardPlan backward_plan(const Shape &p) {
     auto pad = [](int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; };
     const int d2[3] = {p.dim_k, p.dim_k, p.dim_v};
     // One launch of all three where their first dimensions are padded alike -- or where there is so little to do that a
-    // launch more costs more than the wider padding (2 x 1000 tokens of 12 heads of 48 x 80: 57 us, in two launches 65 us; 2 x 2048 of 16 of 64 x 128:
-    // 86 and 94 us; twice that: no difference).
+    // launch more costs more than the wider padding (2 x 1000 tokens of 12 heads of 48 x 80: 55 us, in two launches 67 us;
+    // 2 x 2048 of 16 of 64 x 128: 83 and 93 us; twice that: 126 and 124 us).
     const int wide = std::max(pad(p.dim_k), pad(p.dim_v));
     if (pad(p.dim_k) == pad(p.dim_v) || (wide <= 128 && total_rows(p) * p.heads <= 65536)) {
         bp.launches = 1;

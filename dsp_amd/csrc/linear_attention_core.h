@@ -20,12 +20,13 @@
 // so the state keeps fp32's accuracy over any length (two parts: 6e-7 of it lost for 13 % of the time).  fp32 and fp16
 // samples are multiplied in fp32 (v_mfma_f32_16x16x4_f32): an fp16 state would overflow.
 //
-// What bounds it, at 32,768 tokens x 16 heads of 128 x 128 bf16 (32 segments, two workgroups of four waves a CU): 140 us for
-// 537 MB of q, k, v and o, 3.8 TB/s; the same walk over memory without the arithmetic takes 95 us.  Of the waves' cycles the
-// matrix pipes are busy in 0.2, the vector units in 0.2; the rest waits for LDS, for the partner wave and for memory.  The
-// pass that finds the segments' states: 70 us for 268 MB of k and v.  Measured and not kept: eight waves of 128 registers
-// (160 us), chunks of 32 tokens (three workgroups a CU, spills: 285 us), LDS reads a step ahead of the products (140 us),
-// workgroups dealt to the XCDs by segment (140 us), q and P stored in the order they are read (142 us).
+// What bounds it, at 32,768 tokens x 16 heads of 128 x 128 bf16 (32 segments, two workgroups of four waves a CU): 148 us for
+// 537 MB of q, k, v and o, 3.6 TB/s; the same walk over memory without the arithmetic takes 95 us.  The matrix pipes are busy
+// in a quarter of the SIMDs' cycles, and a wave issues vector instructions in a fifth of its own; the rest waits for LDS, for
+// the partner wave and for memory.  The pass that finds the segments' states: 74 us for 268 MB of k and v.  Measured and not
+// kept, when the same took 140 us: eight waves of 128 registers (160 us), chunks of 32 tokens (three workgroups a CU, spills:
+// 285 us), LDS reads a step ahead of the products (140 us), workgroups dealt to the XCDs by segment (140 us), q and P stored
+// in the order they are read (142 us).
 #pragma once
 
 #include <type_traits>
@@ -373,7 +374,7 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same in all its lanes: branches on it are scalar
     const int d1 = role.d1, d2 = role.d2;
     // fp32 products are a sixteenth as fast as bf16's, and what bounds their kernels: steps behind d1, and waves behind d2,
-    // leave them out (gradients of 11 x 1200 tokens of 14 heads of 192 x 16 in fp16: 476 us, with them 615).
+    // leave them out (gradients of 11 x 1200 tokens of 14 heads of 192 x 16 in fp16: 485 us, with them 621).
     constexpr bool kTrim = sizeof(Tc) == 4;
     const bool busy = n0 + 16 * NT * wave < d2;
     const float log2w = a.log2_decay[head], read = role.read, write = role.write, pscale = role.pscale;
@@ -614,7 +615,7 @@ __device__ __forceinline__ void linear_attention_body(const Args &a, const Role 
 
         // S <- w^size S + K^T (weighted V), the weighted V in three bf16 parts (fp32: in one); rows behind the last are zeros.
         // Every weight is one at most and S is as large as it is: to put the decay off, and to weight V the more for it, would
-        // save 2 to 4 % of the time but lose the largest numbers.
+        // save 2 to 5 % of the time but lose the largest numbers.
         const float hi = more ? whole.hi : rest.hi, lo = more ? whole.lo : rest.lo;
 #pragma unroll
         for (int i = 0; i < DT * NT; ++i)

@@ -3,7 +3,7 @@
 // Bound by the tensor's traffic, read once and written once.  The angle of a pair is the same for every head of a token, and
 // forming it costs more than turning a pair (a double product reduced to turns, then cos and sin in fp32): a thread keeps
 // the angles of its 16 bytes of pairs and turns them in up to kReuse heads.  65,536 tokens of 40 heads of 128 bf16: 248 us
-// for 1.34 GB, 5.4 TB/s (a copy of 1 GiB: 5.1); 64 tokens of 20 heads: 4.2 us, a launch and two latencies.
+// for 1.34 GB, 5.4 TB/s (a copy of 1 GiB: 5.1); 64 tokens of 20 heads: 4.3 us, a launch and two latencies.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>

@@ -15,6 +15,9 @@ Sequence layers (no counterpart in the reference; torch CUDA tensors, fp32, fp16
     linear_attention_backward(q, k, v, log_decay, do) its gradients
     linear_attention_step(q, k, v, log_decay, state)  one token a row, states updated in place
 
+Nothing here is recorded by autograd: outputs of inputs that require gradients have none, and the gradients of the sequence
+layers are calls of their own (rotary with inverse=True, linear_attention_backward), for a torch.autograd.Function to make.
+
 Inputs are torch CUDA tensors (device pointers, asynchronous on the current torch stream)
 or numpy arrays (host pointers, staged by the library).  fp32 unless a name says otherwise.  No CPU fallback.
 """
@@ -434,7 +437,8 @@ def rotary(x, inv_freq, positions=None, position: int = 0, layout: str = "half",
     axis; the first 2 * len(inv_freq) elements of each head are turned by the angle pos * inv_freq (host doubles,
     design.rotary_frequencies), pairs (i, i + half) for layout "half", (2i, 2i + 1) for "interleaved"; the rest is copied.
     positions: int64 [batch, n] or [n] on x's device, or None: position, position + 1, ...  inverse: the other way round --
-    the gradient of the forward call, with the same gain.  out may be x (in place) or any tensor of its shape."""
+    the gradient of the forward call, with the same gain (autograd does not record the call).  out may be x (in place) or any
+    tensor of its shape."""
     kind = _sample_type(x, "x")
     if x.ndim not in (3, 4):
         raise _bad("x must be [batch, n, heads, dim] or [n, heads, dim]")
@@ -530,9 +534,10 @@ def linear_attention(q, k, v, log_decay, scale: float = 1.0, state=None, new_sta
     """Linear attention with a decay for each head (dsp_gpu_linear_attention): S_t = w S_{t-1} + k_t v_t^T and
     o_t = scale * q_t S_t with w = exp(log_decay[head]).  q, k [batch, n, heads, dim_k], v [batch, n, heads, dim_v], heads
     of each a divisor of len(log_decay); any strides with a contiguous last axis.  A packed batch: [rows, heads, dim] with
-    offsets int64 [batch + 1] on the device (max_length: the longest sequence, else all rows); a padded one: lengths int64
-    [batch].  state / new_state: float32 [batch, heads, dim_k, dim_v] before the first and after the last token (may be the
-    same tensor).  Returns o [batch, n, heads, dim_v] (rows of no sequence: zeros, or what `out` held)."""
+    offsets int64 [batch + 1] on the device, not decreasing (max_length: the longest sequence, else all rows; the memory that
+    the call takes is the same); a padded one: lengths int64 [batch].  state / new_state: float32 [batch, heads, dim_k, dim_v]
+    before the first and after the last token (may be the same tensor).  Returns o [batch, n, heads, dim_v] (rows of no
+    sequence: zeros, or what `out` held).  Autograd does not record the call: its gradients are linear_attention_backward."""
     a = _Attention(q, k, v, log_decay, lengths, offsets, max_length, 4)
     o = _new(v, a.out_shape) if out is None else _same(out, q, a.out_shape, "out")
     shape = a.shape(o, "out", out is None)
