@@ -138,3 +138,38 @@ def test_very_many_packed_sequences(ops, dev):
     for i in (0, 1, 31234, 59999, 60000):
         at = slice(int(offsets[i]), int(offsets[i + 1]))
         check_forward(*(x[at][None] for x in (q, k, v)), SLOW, 0.3, None, out[at][None], end[i:i + 1])
+
+
+@pytest.mark.parametrize("most", [None, 700])
+def test_a_captured_packed_call_with_other_offsets(ops, dev, most):
+    """Offsets are data: a captured prompt with its state in place and its gradients, replayed on other sequences, are the eager
+    calls on those -- with joined segments and with few."""
+    h, dk, dv, rows, b = 2, 40, 72, 2100, 5
+    q, k, v, do, _, _ = (x[0] for x in make(dev, torch.bfloat16, 1, rows, h, h, 1, h, dk, dv, seed=15))
+    s0 = torch.randn(b, h, dk, dv, generator=torch.Generator().manual_seed(16)).to(dev)
+    cuts = [[0, 700, 700, 1400, 1401, 2100], [0, 1, 129, 129, 800, 1500], [300, 300, 300, 300, 300, 300], [7, 650, 1206, 1334, 1400, 2093]]
+    offsets, state, ds = torch.tensor(cuts[0], device=dev), s0.clone(), torch.empty_like(s0)
+    more = dict(scale=0.3, offsets=offsets, max_length=most)
+
+    def work():
+        out = ops.linear_attention(q, k, v, SLOW[:h], state=state, new_state=state, **more)
+        return [out, *ops.linear_attention_backward(q, k, v, SLOW[:h], do, state=s0, dnew_state=s0, dstate=ds, **more)]
+
+    work()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for cut in cuts[1:] + cuts:
+        offsets.copy_(torch.tensor(cut))
+        state.copy_(s0)
+        want = [*work(), state.clone(), ds.clone()]
+        state.copy_(s0)
+        ds.fill_(math.nan)
+        for x in got:
+            x.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip([*got, state, ds], want)), cut
+        end = torch.empty_like(s0)
+        ops.linear_attention(q, k, v, SLOW[:h], state=s0, new_state=end, **more)
+        assert torch.equal(state, end), cut
